@@ -417,6 +417,82 @@ int gdn_prefill_segmented_launch(const void* q, const void* k, const void* v, co
                                  size_t workspace_bytes, void* stream);
 
 /*
+ * Softmax attention of the layers that stand between Gated DeltaNet layers (no counterpart
+ * in the reference): per-head norm with rotation, whole prompts, and the newest tokens over
+ * a paged cache.  head_size must be 128; num_q_heads is a multiple (of at most 64) of
+ * num_kv_heads and query head h reads key/value head h / (num_q_heads / num_kv_heads).
+ * Strides are elements between consecutive token rows (or pages), heads dense inside a row
+ * and rows inside a page; rows must not overlap, and every pointer and stride keeps rows
+ * 16-byte aligned (else GDN_ERR_INVALID_ARGUMENT).  scale <= 0 means 1/sqrt(128).
+ *
+ * gdn_attn_qk_norm_rope_launch: for every token and head of q and k,
+ *   y = x * rsqrt(mean(x^2) + eps) * weight    (a NULL weight: y = x)
+ * and the rotation of y's first rotary_dim values (even, 2..128) by the token's row of
+ * rope_table, fp32 [table_rows, rotary_dim]: cosines first, then sines, of the
+ * rotary_dim / 2 pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved != 0:
+ *   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)
+ * in fp32, rounded once.  q bf16 [num_tokens, num_q_heads, 128], k and v bf16 [num_tokens,
+ * num_kv_heads, 128]; q_out like q (may be q).  With k_cache == NULL the rows of k go to
+ * k_out (may be k) and v, slots and v_cache are not used.  Otherwise they go, with v's, to
+ * row slots[t] % page_size of page slots[t] / page_size of k_cache and v_cache (bf16
+ * [num_pages, page_size, num_kv_heads, 128]); slots must be distinct.  A slot outside the
+ * cache writes nothing there.  A position outside [0, table_rows) marks a padding token:
+ * zeros in q_out (and k_out), nothing in the cache.  q_weight, k_weight fp32 [128], 16-byte
+ * aligned.  positions, slots: int32 or int64 [num_tokens].
+ */
+int gdn_attn_qk_norm_rope_launch(const void* q, const void* k, const void* v,
+                                 const void* positions, int positions_int64,
+                                 const float* rope_table, long long table_rows,
+                                 const float* q_weight, const float* k_weight, float eps,
+                                 int interleaved, void* q_out, void* k_out, const void* slots,
+                                 int slots_int64, void* k_cache, void* v_cache,
+                                 long long num_pages, int page_size, long long k_page_stride,
+                                 long long v_page_stride, int num_tokens, int num_q_heads,
+                                 int num_kv_heads, int head_size, int rotary_dim,
+                                 long long q_stride, long long k_stride, long long v_stride,
+                                 long long q_out_stride, long long k_out_stride, void* stream);
+
+/*
+ * Bytes of device workspace the two attention entry points below need (may be 0); 16-byte
+ * aligned scratch, not shared by calls that overlap on the GPU.
+ */
+size_t gdn_attn_workspace_size(int total_q, int num_seqs, int num_q_heads, int num_kv_heads);
+
+/*
+ * Causal attention over packed whole prompts.  q, output bf16 [total_tokens, num_q_heads,
+ * 128], k, v bf16 [total_tokens, num_kv_heads, 128]; cu_seqlens as in gdn_prefill_launch,
+ * but its last entry may lie below total_tokens: the rows behind it are left as they are.
+ */
+int gdn_attn_prefill_launch(const void* q, const void* k, const void* v, const void* cu_seqlens,
+                            int cu_seqlens_int64, float scale, void* output, int total_tokens,
+                            int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                            long long q_stride, long long k_stride, long long v_stride,
+                            long long output_stride, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/*
+ * Causal attention of the newest tokens of each sequence over its paged cache (which holds
+ * them already).  q, output bf16 [total_q, num_q_heads, 128], the tokens of sequence s in
+ * rows cu_seqlens[s] .. cu_seqlens[s + 1] (NULL: total_q / num_seqs tokens each); k_cache,
+ * v_cache bf16 [num_pages, page_size, num_kv_heads, 128], page_size a multiple of 8;
+ * block_table int32 [num_seqs, table_width] (rows block_table_stride entries apart): the
+ * pages of each sequence in order; kv_lens int32 or int64 [num_seqs]: its tokens, the new
+ * ones included (at most table_width * page_size are used).  Token i of q_len sees the
+ * first kv_len - q_len + i + 1 tokens; one that sees none gets zeros.  A page number
+ * outside [0, num_pages) reads as zeros.  What lies behind kv_len in a page is not used,
+ * whatever it holds.
+ */
+int gdn_attn_paged_launch(const void* q, const void* k_cache, const void* v_cache,
+                          const int* block_table, long long block_table_stride,
+                          const void* kv_lens, int kv_lens_int64, const void* cu_seqlens,
+                          int cu_seqlens_int64, float scale, void* output, int total_q,
+                          int num_seqs, int table_width, int num_pages, int page_size,
+                          long long k_page_stride, long long v_page_stride, int num_q_heads,
+                          int num_kv_heads, int head_size, long long q_stride,
+                          long long output_stride, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
  * Diagnostics: synchronises the current device and returns the device-side
  * error bits recorded by the kernels since the last call (0 = none; 1 = a TMA
  * or bulk-copy wait ran out, 2 = a tensor-core wait ran out, 8 = a shared-memory

@@ -10,7 +10,10 @@ MLSys26 FlashInfer contest GDN track:
 exposed as ``decode.kernel`` / ``prefill.kernel``), plus the multi-token decode of
 the ``gdn_mtp`` definition (``gdn_mtp`` / ``mtp_kernel``) for speculative-decoding
 verification over a state pool, and ``chunk_gated_delta_rule`` (FlashInfer's prefill
-argument order: precomputed gates, state checkpoints every N tokens).  All compute runs
+argument order: precomputed gates, state checkpoints every N tokens).  For the
+softmax-attention layers between Gated DeltaNet layers: ``attn_qk_norm_rope`` /
+``attn_append`` (per-head norm and rotation, into the paged cache), ``attn_prefill``
+(packed prompts) and ``attn_paged`` (the newest tokens over the cache).  All compute runs
 in the in-tree CUDA library ``libgdn_b200.so`` through its C ABI
 (``include/gdn_b200.h``); importing this package fails if it is not built.
 
@@ -22,10 +25,13 @@ from .decode import gdn_decode, kernel as decode_kernel  # noqa: F401
 from .prefill import (chunk_gated_delta_rule, gdn_prefill, gdn_prefill_recurrent,  # noqa: F401
                       gdn_prefill_segmented, kernel as prefill_kernel, workspace_bytes)
 from .mtp import gdn_mtp, kernel as mtp_kernel  # noqa: F401
-from . import decode, mtp, prefill, sharding, workloads  # noqa: F401
+from .rope import attn_append, attn_qk_norm_rope, rope_table  # noqa: F401
+from .attention import attn_paged, attn_prefill  # noqa: F401
+from . import attention, decode, mtp, prefill, rope, sharding, workloads  # noqa: F401
 
 __all__ = ["gdn_decode", "gdn_prefill", "gdn_prefill_recurrent", "gdn_prefill_segmented",
            "gdn_mtp", "decode_kernel",
            "mtp_kernel", "chunk_gated_delta_rule",
+           "attn_qk_norm_rope", "attn_append", "attn_prefill", "attn_paged", "rope_table",
            "prefill_kernel", "workloads", "sharding", "GDNError", "LIB", "LIB_PATH", "workspace_bytes",
            "device_error"]

@@ -114,3 +114,54 @@ def scale_arg(scale) -> float:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def attn_heads(hq: int, hk: int, d: int) -> None:
+    if d != HEAD_SIZE:
+        raise ValueError(f"head_size must be {HEAD_SIZE}, got {d}")
+    if hk <= 0 or hq < hk or hq % hk != 0 or hq // hk > 64:
+        raise ValueError(f"the query heads ({hq}) must be 1 to 64 times the key/value heads ({hk})")
+
+
+def paged_cache(k_cache, v_cache, hk: int, device: torch.device):
+    """Elements between the pages of k_cache and v_cache [num_pages, page_size, hk, 128]:
+    dense pages, 16-byte aligned, that do not overlap (updated in place, so never copied)."""
+    strides = []
+    for name, x in (("k_cache", k_cache), ("v_cache", v_cache)):
+        tensor(name, x, torch.bfloat16, 4, device, strided=True)
+        if x.shape[0] < 1 or x.shape[1] < 1:
+            raise ValueError(f"{name} must have at least one page, got shape {tuple(x.shape)}")
+        shape(name, x, (k_cache.shape[0], k_cache.shape[1], hk, HEAD_SIZE))
+        rs = row_stride(x, 8)
+        if rs is None or x.data_ptr() % 16 != 0:
+            raise ValueError(f"{name}'s pages must be dense, 16-byte aligned and must not overlap")
+        strides.append(rs)
+    return strides
+
+
+def token_rows(x: torch.Tensor):
+    """x [B, T, H, D] as [B * T, H, D] rows that are one stride apart; None if they are not."""
+    B, T = x.shape[:2]
+    if B > 1 and T > 1 and x.stride(0) != T * x.stride(1):
+        return None
+    if T == 1:
+        return x[:, 0]
+    return x.view(B * T, *x.shape[2:]) if B == 1 or x.stride(0) == T * x.stride(1) else None
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one (nothing is done if it is already)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)

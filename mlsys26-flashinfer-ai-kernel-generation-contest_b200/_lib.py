@@ -61,6 +61,14 @@ SIGNATURES = {
     "gdn_prefill_segmented_launch": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _vp,
                                           _i, _i, _i, _i, _i, _i, _i, _vp, _ll, _ll, _ll, _ll,
                                           _ll, _vp, _sz, _vp]),
+    "gdn_attn_qk_norm_rope_launch": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _ll, _vp, _vp, _f, _i,
+                                          _vp, _vp, _vp, _i, _vp, _vp, _ll, _i, _ll, _ll, _i, _i,
+                                          _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _vp]),
+    "gdn_attn_workspace_size": (_sz, [_i, _i, _i, _i]),
+    "gdn_attn_prefill_launch": (_i, [_vp, _vp, _vp, _vp, _i, _f, _vp, _i, _i, _i, _i, _i, _ll,
+                                     _ll, _ll, _ll, _vp, _sz, _vp]),
+    "gdn_attn_paged_launch": (_i, [_vp, _vp, _vp, _vp, _ll, _vp, _i, _vp, _i, _f, _vp, _i, _i, _i,
+                                   _i, _i, _ll, _ll, _i, _i, _i, _ll, _ll, _vp, _sz, _vp]),
     "gdn_device_error": (_i, [_i]),
     "gdn_selftest_bounded_wait": (_i, [ctypes.c_uint, _i, _vp, _vp]),
 }

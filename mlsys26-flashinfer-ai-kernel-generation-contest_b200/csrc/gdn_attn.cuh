@@ -1,0 +1,71 @@
+// Internal interface of the softmax-attention kernels (packed prompts, paged cache).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+
+#include "gdn_common.cuh"
+
+namespace gdn {
+
+// One call: the newest q_len tokens of each sequence against its kv_len tokens (those
+// included), causal.  Packed prompts: kv rows are the token rows themselves; paged: row j
+// of sequence s is row j % page_size of page block_table[s][j / page_size].
+struct AttnArgs {
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16* out;
+  const void* cu;  // [num_seqs + 1] (null: every sequence has total_q / num_seqs tokens)
+  bool cu64;
+  bool paged;
+  const int* block_table;
+  const void* kv_lens;
+  bool kv64;
+  long long table_stride;  // entries between the rows of block_table
+  int table_width;         // pages a sequence can have
+  int page_size;
+  long long num_pages;
+  long long k_page_stride, v_page_stride;  // elements
+  long long q_stride, k_stride, v_stride, o_stride;
+  long long total_q;
+  int num_seqs, hq, hkv;
+  float scale_log2;  // scale * log2(e)
+};
+
+__device__ __forceinline__ long long attn_index(const void* p, bool is64, long long i) {
+  return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+}
+
+// A sequence's rows, kept inside the buffers whatever cu_seqlens and kv_lens hold.
+struct AttnSeq {
+  long long q0;  // first query row
+  int q_len, kv_len;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& p, int s) {
+  AttnSeq r;
+  long long a, b;
+  if (p.cu != nullptr) {
+    a = attn_index(p.cu, p.cu64, s);
+    b = attn_index(p.cu, p.cu64, s + 1);
+  } else {
+    const long long per = p.total_q / p.num_seqs;
+    a = s * per;
+    b = a + per;
+  }
+  a = a < 0 ? 0 : (a > p.total_q ? p.total_q : a);
+  b = b < a ? a : (b > p.total_q ? p.total_q : b);
+  r.q0 = a;
+  r.q_len = (int)(b - a);
+  if (!p.paged) {
+    r.kv_len = r.q_len;
+  } else {
+    const long long most = (long long)p.table_width * p.page_size;
+    long long n = attn_index(p.kv_lens, p.kv64, s);
+    r.kv_len = (int)(n < 0 ? 0 : (n > most ? most : n));
+  }
+  return r;
+}
+
+cudaError_t launch_attn_simple(const AttnArgs& p, cudaStream_t st);
+
+}  // namespace gdn

@@ -1,0 +1,275 @@
+// Per-head RMSNorm of queries and keys, the position rotation, and the write of keys and
+// values to the paged cache, in one pass (the softmax-attention layers that stand between
+// Gated DeltaNet layers; no counterpart in the reference).
+//
+// For a row x of 128 values (one token, one head), weights w and the table row (c, s) of
+// the token's position:
+//   y = x * rsqrt(mean(x^2) + eps) * w              (without weights: y = x)
+//   (y_a, y_b) -> (y_a c_i - y_b s_i, y_b c_i + y_a s_i)   for the rd / 2 pairs
+// with pairs (i, i + rd/2) or, interleaved, (2i, 2i + 1); values from rd on pass through.
+// Everything is fp32 and rounded once, to bf16, at the end.  The angles come from a table
+// because a position times a frequency loses the angle in 32 bits at far positions (a
+// 2^-24 relative error of 10^6 radians is 0.06); the caller computes it once in 64 bits.
+//
+// Bound by HBM: 256 bytes in and out per row, one table row per token.  16 lanes own a row
+// (16-byte accesses); the sum of squares is four shuffles, the partner of a value in the
+// half layout one shuffle when rd / 2 is a multiple of 8, else a pass through shared memory.
+#include "gdn_common.cuh"
+
+namespace gdn {
+namespace {
+
+struct RopeArgs {
+  const __nv_bfloat16 *q, *k, *v;
+  const void* positions;
+  const float* table;
+  const float *q_weight, *k_weight;  // null: no normalisation
+  __nv_bfloat16 *q_out, *k_out;
+  const void* slots;
+  __nv_bfloat16 *k_cache, *v_cache;  // null: k_out is written instead
+  long long q_stride, k_stride, v_stride, qo_stride, ko_stride;
+  long long k_page_stride, v_page_stride, num_slots, table_rows;
+  long long groups;  // tokens * groups of heads
+  float eps;
+  int hq, hkv, rd, page_size, groups_per_token;
+  bool pos64, slot64;
+};
+
+__device__ __forceinline__ long long load_index(const void* p, bool is64, long long i) {
+  return is64 ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+}
+
+__device__ __forceinline__ float sum16(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 1);
+  x += __shfl_xor_sync(0xffffffffu, x, 2);
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x;
+}
+
+enum RopeLayout { kInterleaved = 0, kHalfAligned = 1, kHalfAny = 2 };
+
+// One half-warp per group of HPG heads of one token: the table row is read once for them
+// and their loads are in flight together.
+template <int HPG, int LAYOUT>
+__global__ void __launch_bounds__(256) rope_kernel(const RopeArgs p) {
+  __shared__ float stage[LAYOUT == kHalfAny ? 16 : 1][kHeadDim];
+  const int lane = threadIdx.x & 15;
+  const long long group = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const bool live = group < p.groups;
+  // lanes of a dead half-warp go along with the shuffles on group 0's values
+  const long long g = live ? group : 0;
+  const long long t = g / p.groups_per_token;
+  const int h0 = (int)(g - t * p.groups_per_token) * HPG;
+  const int heads = p.hq + p.hkv + (p.k_cache != nullptr ? p.hkv : 0);
+
+  uint4 raw[HPG];
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    const int h = h0 + i;
+    const __nv_bfloat16* src =
+        h < p.hq ? p.q + t * p.q_stride + (long long)h * kHeadDim
+        : h < p.hq + p.hkv
+            ? p.k + t * p.k_stride + (long long)(h - p.hq) * kHeadDim
+            : p.v + t * p.v_stride + (long long)(h - p.hq - p.hkv) * kHeadDim;
+    raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + 8 * lane) : make_uint4(0, 0, 0, 0);
+  }
+
+  const long long pos = load_index(p.positions, p.pos64, t);
+  const bool known = pos >= 0 && pos < p.table_rows;  // else: a padding token
+  long long slot = -1;
+  if (p.k_cache != nullptr && known) {
+    slot = load_index(p.slots, p.slot64, t);
+    if (slot >= p.num_slots) slot = -1;
+  }
+  const long long page = slot >= 0 ? slot / p.page_size : 0;
+  const long long off = slot >= 0 ? slot - page * p.page_size : 0;
+
+  // cos / sin of the lane's 8 values (1, 0 where nothing turns)
+  const int half = p.rd >> 1;
+  float c[8], s[8];
+  const float* row = p.table + (known ? pos : 0) * (long long)p.rd;  // not read unless known
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = 8 * lane + e;
+    const int i = LAYOUT == kInterleaved ? d >> 1 : (d < half ? d : d - half);
+    const bool turns = known && d < p.rd;
+    c[e] = turns ? __ldg(row + i) : 1.f;
+    s[e] = turns ? __ldg(row + half + i) : 0.f;
+    // the first of a pair takes -s of the second
+    if (LAYOUT == kInterleaved ? (d & 1) == 0 : d < half) s[e] = -s[e];
+  }
+  // half layout: the lane that holds the partners
+  const int step = half >> 3;
+  const int partner = 8 * lane < half ? lane + step : (8 * lane < p.rd ? lane - step : lane);
+
+#pragma unroll
+  for (int i = 0; i < HPG; ++i) {
+    const int h = h0 + i;
+    const bool is_v = h >= p.hq + p.hkv;
+    float x[8];
+    {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = bf2x2_to_f2(w[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      }
+    }
+    const float* weight = h < p.hq ? p.q_weight : p.k_weight;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    ss = sum16(ss);
+    if (weight != nullptr && !is_v) {
+      const float r = rsqrtf(ss * (1.f / kHeadDim) + p.eps);
+      const float4 w0 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane);
+      const float4 w1 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane + 1);
+      x[0] *= r * w0.x; x[1] *= r * w0.y; x[2] *= r * w0.z; x[3] *= r * w0.w;
+      x[4] *= r * w1.x; x[5] *= r * w1.y; x[6] *= r * w1.z; x[7] *= r * w1.w;
+    }
+    float y[8];
+    if constexpr (LAYOUT == kInterleaved) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+    } else if constexpr (LAYOUT == kHalfAligned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner, 16);
+    } else {
+      float* st = stage[threadIdx.x >> 4];
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st[8 * lane + e] = x[e];
+      __syncwarp();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = 8 * lane + e;
+        y[e] = d < p.rd ? st[d < half ? d + half : d - half] : 0.f;
+      }
+    }
+    uint4 o;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 8 * lane + 2 * e;  // rd is even: both values turn or neither does
+      const float a = d < p.rd ? fmaf(x[2 * e], c[2 * e], y[2 * e] * s[2 * e]) : x[2 * e];
+      const float b = d < p.rd ? fmaf(x[2 * e + 1], c[2 * e + 1], y[2 * e + 1] * s[2 * e + 1])
+                               : x[2 * e + 1];
+      const __nv_bfloat162 b2 = __floats2bfloat162_rn(a, b);
+      w[e] = *reinterpret_cast<const uint32_t*>(&b2);
+    }
+    o = is_v ? raw[i] : known ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0, 0, 0, 0);
+    if (!live || h >= heads) continue;
+    __nv_bfloat16* dst;
+    if (h < p.hq) {
+      dst = p.q_out + t * p.qo_stride + (long long)h * kHeadDim;
+    } else if (p.k_cache == nullptr) {
+      dst = p.k_out + t * p.ko_stride + (long long)(h - p.hq) * kHeadDim;
+    } else {
+      if (slot < 0) continue;
+      dst = is_v ? p.v_cache + page * p.v_page_stride +
+                       (off * p.hkv + (h - p.hq - p.hkv)) * (long long)kHeadDim
+                 : p.k_cache + page * p.k_page_stride +
+                       (off * p.hkv + (h - p.hq)) * (long long)kHeadDim;
+    }
+    *reinterpret_cast<uint4*>(dst + 8 * lane) = o;
+  }
+}
+
+template <int HPG>
+cudaError_t launch_rope(const RopeArgs& p, int layout, cudaStream_t st) {
+  const unsigned grid = (unsigned)((p.groups + 15) / 16);
+  if (layout == kInterleaved)
+    rope_kernel<HPG, kInterleaved><<<grid, 256, 0, st>>>(p);
+  else if (layout == kHalfAligned)
+    rope_kernel<HPG, kHalfAligned><<<grid, 256, 0, st>>>(p);
+  else
+    rope_kernel<HPG, kHalfAny><<<grid, 256, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+inline bool misaligned(const void* p, uintptr_t n) {
+  return (reinterpret_cast<uintptr_t>(p) % n) != 0;
+}
+
+}  // namespace
+}  // namespace gdn
+
+extern "C" int gdn_attn_qk_norm_rope_launch(
+    const void* q, const void* k, const void* v, const void* positions, int positions_int64,
+    const float* rope_table, long long table_rows, const float* q_weight, const float* k_weight,
+    float eps, int interleaved, void* q_out, void* k_out, const void* slots, int slots_int64,
+    void* k_cache, void* v_cache, long long num_pages, int page_size, long long k_page_stride,
+    long long v_page_stride, int num_tokens, int num_q_heads, int num_kv_heads, int head_size,
+    int rotary_dim, long long q_stride, long long k_stride, long long v_stride,
+    long long q_out_stride, long long k_out_stride, void* stream) {
+  using namespace gdn;
+  const long long D = kHeadDim;
+  if (num_tokens < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || table_rows < 0 || !(eps >= 0.f))
+    return GDN_ERR_INVALID_ARGUMENT;
+  if (head_size != kHeadDim || num_q_heads % num_kv_heads != 0 || rotary_dim < 2 ||
+      rotary_dim > kHeadDim || (rotary_dim & 1) != 0)
+    return GDN_ERR_UNSUPPORTED;
+  if (num_q_heads > (1 << 16)) return GDN_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return GDN_OK;
+  const bool cached = k_cache != nullptr;
+  if (!q || !k || !positions || (!rope_table && table_rows > 0) || !q_out)
+    return GDN_ERR_INVALID_ARGUMENT;
+  if (cached ? (!v || !v_cache || !slots) : !k_out) return GDN_ERR_INVALID_ARGUMENT;
+  const long long qw = num_q_heads * D, kw = num_kv_heads * D;
+  auto bad_rows = [](const void* p, long long stride, long long width) {
+    return misaligned(p, 16) || stride < width || stride % 8 != 0;
+  };
+  if (bad_rows(q, q_stride, qw) || bad_rows(k, k_stride, kw) || bad_rows(q_out, q_out_stride, qw) ||
+      misaligned(positions, positions_int64 ? 8 : 4) || misaligned(rope_table, 4) ||
+      misaligned(q_weight, 16) || misaligned(k_weight, 16))
+    return GDN_ERR_INVALID_ARGUMENT;
+  if (cached) {
+    if (num_pages < 0 || page_size <= 0 || bad_rows(v, v_stride, kw) ||
+        bad_rows(k_cache, k_page_stride, page_size * kw) ||
+        bad_rows(v_cache, v_page_stride, page_size * kw) || misaligned(slots, slots_int64 ? 8 : 4))
+      return GDN_ERR_INVALID_ARGUMENT;
+  } else if (bad_rows(k_out, k_out_stride, kw)) {
+    return GDN_ERR_INVALID_ARGUMENT;
+  }
+  using B16 = __nv_bfloat16;
+  RopeArgs p{};
+  p.q = static_cast<const B16*>(q);
+  p.k = static_cast<const B16*>(k);
+  p.v = static_cast<const B16*>(v);
+  p.positions = positions;
+  p.table = rope_table;
+  p.q_weight = q_weight;
+  p.k_weight = k_weight;
+  p.q_out = static_cast<B16*>(q_out);
+  p.k_out = static_cast<B16*>(k_out);
+  p.slots = slots;
+  p.k_cache = static_cast<B16*>(k_cache);
+  p.v_cache = static_cast<B16*>(v_cache);
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.qo_stride = q_out_stride;
+  p.ko_stride = k_out_stride;
+  p.k_page_stride = k_page_stride;
+  p.v_page_stride = v_page_stride;
+  p.num_slots = cached ? num_pages * page_size : 0;
+  p.table_rows = table_rows;
+  p.eps = eps;
+  p.hq = num_q_heads;
+  p.hkv = num_kv_heads;
+  p.rd = rotary_dim;
+  p.page_size = cached ? page_size : 1;
+  p.pos64 = positions_int64 != 0;
+  p.slot64 = slots_int64 != 0;
+  const int heads = num_q_heads + num_kv_heads * (cached ? 2 : 1);
+  const int layout =
+      interleaved ? kInterleaved : (rotary_dim % 16 == 0 ? kHalfAligned : kHalfAny);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  constexpr int hpg = 4;
+  p.groups_per_token = (heads + hpg - 1) / hpg;
+  p.groups = (long long)num_tokens * p.groups_per_token;
+  if ((p.groups + 15) / 16 > 0x7fffffffLL) return GDN_ERR_INVALID_ARGUMENT;
+  return launch_rope<hpg>(p, layout, st) == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+}

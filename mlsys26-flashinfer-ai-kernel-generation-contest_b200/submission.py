@@ -38,7 +38,7 @@ OPS = {
     "gdn_mtp": ("mtp_kernel", "gdn_mtp_qk16_v32_d128_k_last"),
 }
 PY_FILES = ("__init__.py", "_lib.py", "_checks.py", "decode.py", "prefill.py", "mtp.py",
-            "sharding.py", "workloads.py", "build.py")
+            "rope.py", "attention.py", "sharding.py", "workloads.py", "build.py")
 
 KERNEL_PY = '''"""flashinfer-bench entry point for {op}: B200 (sm_100a) Gated DeltaNet kernels.
 
