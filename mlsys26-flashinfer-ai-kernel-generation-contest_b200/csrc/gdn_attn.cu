@@ -2,7 +2,7 @@
 // of the kernel.
 #include <cmath>
 
-#include "gdn_attn.cuh"
+#include "gdn_attn_sched.cuh"
 
 namespace gdn {
 namespace {
@@ -22,12 +22,27 @@ bool bad_rows(const void* p, long long stride, long long width) {
   return !p || misaligned(p, 16) || stride < width || stride % 8 != 0;
 }
 
+// CTAs of a launch: one per SM of the current device (without one: what a size needs at most).
+constexpr int kMaxParts = 160;
+int parts() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0 ||
+      n > kMaxParts)
+    n = kMaxParts;
+  return n;
+}
+
+size_t workspace_size() { return attn_partial_bytes(attn_tc_rows(), kMaxParts); }
+
 int launch(AttnArgs& p, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
+  if (!workspace || workspace_bytes < workspace_size()) return GDN_ERR_WORKSPACE;
+  if (misaligned(workspace, 16)) return GDN_ERR_INVALID_ARGUMENT;
   p.scale_log2 = default_scale(scale) * 1.4426950408889634f;
-  return launch_attn_simple(p, static_cast<cudaStream_t>(stream)) == cudaSuccess ? GDN_OK
-                                                                                 : GDN_ERR_LAUNCH;
+  return launch_attn_tc(p, parts(), static_cast<float*>(workspace),
+                        static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? GDN_OK
+             : GDN_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -39,7 +54,7 @@ extern "C" size_t gdn_attn_workspace_size(int total_q, int num_seqs, int num_q_h
   (void)num_seqs;
   (void)num_q_heads;
   (void)num_kv_heads;
-  return 0;
+  return gdn::workspace_size();
 }
 
 extern "C" int gdn_attn_prefill_launch(const void* q, const void* k, const void* v,

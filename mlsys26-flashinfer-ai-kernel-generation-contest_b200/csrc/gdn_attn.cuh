@@ -66,6 +66,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& p, int s) {
   return r;
 }
 
-cudaError_t launch_attn_simple(const AttnArgs& p, cudaStream_t st);
+// Tensor-core kernel on `sms` CTAs (workspace: attn_partial_bytes(attn_tc_rows(), sms)).
+int attn_tc_rows();
+cudaError_t launch_attn_tc(const AttnArgs& p, int sms, float* workspace, cudaStream_t st);
 
 }  // namespace gdn

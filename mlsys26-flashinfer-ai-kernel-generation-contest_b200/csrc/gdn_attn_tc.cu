@@ -1,0 +1,626 @@
+// Causal softmax attention on the tensor cores: packed prompts and chunks over a paged cache.
+//
+//   S = scale Q K^T,  P = 2^(S - m),  l = sum P,  O = P V / l
+// over tiles of 128 keys with a running maximum m per row.  A tile of 128 rows holds the
+// query heads of one key/value head for 128 / group tokens (all of them read the same keys),
+// and a CTA works on two such tiles, in turn: while one's scores go through the exponential
+// (16 per clock and SM), the tensor cores multiply for the other.
+//
+// Warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, scores read from TMEM and
+// P written back over them as the bf16 A operand of the second product.  Warp 8: issues the
+// products.  Warp 9: loads K and V tiles by TMA into a ring of five (K and V in turn), Q once
+// per item.  (Warps 10 and 11 fill the register group.)  TMEM: S0 S1 O0 O1, 128 columns each.
+//
+// The maximum that a row's sums are relative to is raised only when the new one exceeds it
+// by 2^8: P then stays below 2^8 and the sums in fp32 lose nothing, and the rescaling of O
+// (a round trip through the registers) is rare.  The sum l adds the fp32 values of P; the
+// product takes them rounded to bf16 (relative 2^-8, as the output's own rounding).
+//
+// Key rows behind kv_len in a sequence's last tile can hold anything: their scores are
+// replaced, and their rows of V are zeroed in shared memory (0 * inf is not 0).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "gdn_attn_sched.cuh"
+#include "gdn_prefill.cuh"
+#include "sm100.cuh"
+
+namespace gdn {
+namespace {
+
+using namespace sm100;
+
+constexpr int kRows = 128;             // rows of a tile
+constexpr int kTile = 128;             // keys of a tile
+constexpr int kStages = 5;             // K / V ring
+constexpr int kHalfBytes = 128 * 128;  // 64 columns of 128 rows, 128-byte swizzle
+constexpr int kTileBytes = 2 * kHalfBytes;
+constexpr int kThreads = 384;          // 168 registers a thread at launch: 64512
+// the softmax warps hold a row of scores: 256 x 216 + 128 x 72 registers = 64512
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
+constexpr float kRaise = 8.f;  // log2 of how far the maximum may be exceeded
+
+__device__ unsigned int g_attn_error = 0;
+constexpr unsigned kErrLoad = 1u, kErrTensor = 2u;
+
+constexpr int kWorks = 2;  // items handed out ahead
+struct Bars {
+  uint64_t q_full[2], q_empty;
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint64_t work_full[kWorks], work_empty[kWorks];
+  uint64_t drain;
+};
+// One piece of an item, for all roles.
+struct Work {
+  long long row0;  // query row of the block's first token
+  int seq, head;
+  int toks;        // tokens of the block
+  int kv0, kv_len;  // first key row (packed prompts), keys of the sequence
+  int lim0;        // keys that the block's first token sees (may be negative); one more each
+  int t0, t1;      // key tiles of the piece
+  int end[2];      // of which row tile 0 / 1 needs those below
+  int slot;        // partial results' slot, -1: the piece is the whole item
+  bool live;       // false: behind the last one
+};
+struct Shared {
+  Bars bars;
+  AttnShare share;
+  Work work[kWorks];
+  uint32_t tmem;
+  int failed;
+};
+constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + kStages * kTileBytes;
+
+struct TcArgs {
+  AttnArgs a;
+  AttnGrid g;
+  float* ws;
+  int box;  // key rows per TMA box
+};
+
+// The piece of item `cur` inside [u0, u1); false if there is none.
+__device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& g, long long u0,
+                                         long long u1, Work* w) {
+  const int e = cur.keys(g);
+  const int n = (e + kTile - 1) / kTile;
+  const int t0 = attn_tile_at(g, e, n, u0 > cur.start ? u0 - cur.start : 0);
+  const int t1 = attn_tile_at(g, e, n, u1 - cur.start);
+  // an item without keys belongs to the CTA that it starts in (its rows are zeroed)
+  if (t1 <= t0 && !(n == 0 && cur.start >= u0)) return false;
+  const int first = cur.b * g.block;
+  w->row0 = cur.seq.q0 + first;
+  w->seq = cur.s;
+  w->head = cur.h;
+  w->toks = min(g.block, cur.seq.q_len - first);
+  w->kv0 = (int)cur.seq.q0;
+  w->kv_len = cur.seq.kv_len;
+  w->lim0 = cur.seq.kv_len - cur.seq.q_len + first + 1;
+  w->t0 = t0;
+  w->t1 = t1;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {  // a row tile sees what its last token sees
+    const int toks = min(w->toks - t * g.sub, g.sub);
+    const int sees = toks > 0 ? w->lim0 + t * g.sub + toks - 1 : 0;
+    w->end[t] = min(t1, sees > 0 ? (sees + kTile - 1) / kTile : 0);
+  }
+  w->slot = (t0 == 0 && t1 == n) ? -1 : (u0 > cur.start ? 0 : 1);
+  w->live = true;
+  return true;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint64_t* bar,
+                                            int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&b);
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                   const __grid_constant__ CUtensorMap mv, const TcArgs p) {
+  extern __shared__ uint8_t raw[];
+  __shared__ Shared sh;
+  uint8_t* tiles = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t sq = smem_u32(tiles);
+  const uint32_t skv = sq + 2 * kTileBytes;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const AttnArgs& a = p.a;
+  const AttnGrid& g = p.g;
+  const int grp = a.hq / a.hkv;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    Bars& b = sh.bars;
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&b.q_full[t], 1);
+      mbar_init(&b.s_full[t], 1);
+      mbar_init(&b.p_ready[t], 128);
+      mbar_init(&b.o_full[t], 1);
+    }
+    mbar_init(&b.q_empty, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&b.kv_full[i], 1);
+      mbar_init(&b.kv_empty[i], 1);
+    }
+    for (int i = 0; i < kWorks; ++i) {
+      mbar_init(&b.work_full[i], 1);
+      mbar_init(&b.work_empty[i], 10);  // loader, issuer, eight softmax warps
+    }
+    mbar_init(&b.drain, 1);
+    fence_mbar_init();
+    sh.failed = 0;
+    tma_prefetch_desc(&mq);
+    tma_prefetch_desc(&mk);
+    tma_prefetch_desc(&mv);
+  }
+  if (warp == 8) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  attn_share<kThreads>(a, g, blockIdx.x, gridDim.x, &sh.share);  // ends with __syncthreads
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  volatile int* failed = &sh.failed;
+  Bars& bars = sh.bars;
+
+  // Every role takes the same pieces in the same order.  K tile i of the CTA is ring entry
+  // 2 i, its V entry 2 i + 1.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 10) {
+      // ------------------------------------------------------------------ the pieces
+      if (lane == 0) {
+        const long long u0 = sh.share.u0;
+        const long long u1 = attn_cut(sh.share.total, blockIdx.x + 1, gridDim.x);
+        AttnCursor cur;
+        bool more = u0 < u1;
+        if (more) cur.seek(a, g, sh.share.seq, sh.share.seq_start, u0);
+        uint32_t n = 0;
+        bool ok = true;
+        while (ok) {
+          if (n >= kWorks) ok = mbar_wait(&bars.work_empty[n % kWorks], (n / kWorks - 1) & 1);
+          if (!ok || *failed) break;
+          Work* w = &sh.work[n % kWorks];
+          bool found = false;
+          while (more && !found) {
+            found = piece_of(cur, g, u0, u1, w);
+            more = cur.next(a, g) && cur.start < u1;
+          }
+          if (!found) w->live = false;
+          mbar_arrive(&bars.work_full[n % kWorks]);
+          if (!found) break;
+          ++n;
+        }
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------ loads
+      uint32_t ring = 0, items = 0;
+      bool ok = true;
+      for (uint32_t n = 0;; ++n) {
+        ok = mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1);
+        const Work w = sh.work[n % kWorks];
+        __syncwarp();
+        if (!ok || !w.live || *failed) break;
+        if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
+        if (w.t1 <= w.t0) continue;
+        if (items > 0) ok = mbar_wait(&bars.q_empty, (items - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          for (int t = 0; t < 2; ++t) {
+            if (w.end[t] <= w.t0) continue;  // the row tile has nothing to do
+            mbar_arrive_expect_tx(&bars.q_full[t], 2 * g.sub * grp * 128);
+            for (int h = 0; h < 2; ++h)
+              tma_load_3d(sq + t * kTileBytes + h * kHalfBytes, &mq, &bars.q_full[t], 64 * h,
+                          w.head * grp, (int)w.row0 + t * g.sub);
+          }
+        }
+        ++items;
+        const int* table = a.paged ? a.block_table + w.seq * a.table_stride : nullptr;
+        const int x = w.head * kHeadDim;
+        for (int j = w.t0; j < w.t1 && ok; ++j) {
+          for (int kv = 0; kv < 2; ++kv) {
+            const uint32_t st = ring % kStages;
+            if (ring >= kStages) ok = mbar_wait(&bars.kv_empty[st], (ring / kStages - 1) & 1);
+            ok = ok && !*failed;
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[st], kTileBytes);
+            __syncwarp();
+            const uint32_t dst = skv + st * kTileBytes;
+            const CUtensorMap* m = kv ? &mv : &mk;
+            for (int i = lane; i < kTile / p.box; i += 32) {
+              const int key = j * kTile + i * p.box;
+              int row, page;
+              if (table == nullptr) {
+                row = w.kv0 + key;
+                page = 0;
+              } else {
+                row = key % a.page_size;
+                page = key < w.kv_len ? __ldg(table + key / a.page_size) : -1;  // -1: not used
+                if (page < 0 || page >= a.num_pages) page = -1;  // no such page: zeros
+              }
+              for (int h = 0; h < 2; ++h)
+                tma_load_3d(dst + h * kHalfBytes + i * p.box * 128, m, &bars.kv_full[st],
+                            x + 64 * h, row, page);
+            }
+            ++ring;
+          }
+        }
+        if (!ok) break;
+      }
+      if (!ok) {
+        *failed = 1;
+        if (lane == 0) atomicOr(&g_attn_error, kErrLoad);
+      }
+      if (!ok || *failed) {
+        // copies in flight write into this block's memory: wait for them before it ends
+        for (uint32_t i = ring > kStages ? ring - kStages : 0; i < ring; ++i)
+          mbar_wait(&bars.kv_full[i % kStages], (i / kStages) & 1, 1u << 20);
+      }
+    } else if (warp == 8) {
+      // ------------------------------------------------------------------ products
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false);
+        constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
+        uint32_t tile0 = 0;             // K / V tiles before this piece
+        uint32_t np0 = 0, np1 = 0;      // p_ready phases used
+        uint32_t nq0 = 0, nq1 = 0;      // q_full phases used
+        bool ok = true;
+        unsigned why = 0;
+        auto wait = [&](uint64_t* bar, uint32_t phase, unsigned err) {
+          if (!ok) return;
+          ok = mbar_wait(bar, phase & 1);
+          if (!ok) why = err;
+          if (*failed) ok = false;
+        };
+        auto scores = [&](int t, uint32_t entry) {  // S_t = Q_t K^T
+          const uint32_t k = skv + entry % kStages * kTileBytes;
+          const uint32_t q = sq + t * kTileBytes;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t off = (i >> 2) * kHalfBytes + (i & 3) * 32;
+            umma_bf16(tmem + 128 * t, umma_desc_k(q + off), umma_desc_k(k + off), idesc_s, i > 0);
+          }
+          umma_commit(&bars.s_full[t]);
+        };
+        auto values = [&](int t, uint32_t entry, bool first) {  // O_t += P_t V
+          const uint32_t v = skv + entry % kStages * kTileBytes;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            umma_bf16_tmem_a(tmem + 256 + 128 * t, tmem + 128 * t + 8 * i,
+                             umma_desc_mn(v + i * 2048, kHalfBytes), idesc_o, !first || i > 0);
+        };
+        for (uint32_t n = 0; ok; ++n) {
+          wait(&bars.work_full[n % kWorks], n / kWorks, kErrLoad);
+          if (!ok || !sh.work[n % kWorks].live) break;
+          const int t0 = sh.work[n % kWorks].t0, t1 = sh.work[n % kWorks].t1;
+          const int end0 = sh.work[n % kWorks].end[0], end1 = sh.work[n % kWorks].end[1];
+          mbar_arrive(&bars.work_empty[n % kWorks]);
+          if (t1 <= t0) continue;
+          // the row tile that holds the block's last token needs every key tile: it comes last
+          // and releases what both have read
+          const int last = end1 == t1 ? 1 : 0;
+          uint32_t entry = 2 * tile0;
+          wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
+          auto begin = [&](int t) {  // scores of tile j into S_t; K and, at the end, Q released
+            scores(t, entry);
+            if (t == last) umma_commit(&bars.kv_empty[entry % kStages]);
+          };
+          if (end0 > t0) {
+            wait(&bars.q_full[0], nq0++, kErrLoad);
+            if (!ok) break;
+            tc_fence_after();
+            begin(0);
+          }
+          if (end1 > t0) {
+            wait(&bars.q_full[1], nq1++, kErrLoad);
+            if (!ok) break;
+            tc_fence_after();
+            begin(1);
+          }
+          if (t0 + 1 == t1) umma_commit(&bars.q_empty);
+          for (int j = t0; j < t1 && ok; ++j) {
+            const uint32_t ve = entry + 1;  // V of tile j; the K of tile j + 1 comes behind it
+            entry += 2;
+            wait(&bars.kv_full[ve % kStages], ve / kStages, kErrLoad);
+            if (j + 1 < t1) wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
+            if (j < end0) {
+              wait(&bars.p_ready[0], np0++, kErrTensor);
+              if (!ok) break;
+              tc_fence_after();
+              values(0, ve, j == t0);
+              if (last == 0) umma_commit(&bars.kv_empty[ve % kStages]);
+              if (j + 1 < end0) begin(0);
+              else umma_commit(&bars.o_full[0]);
+            }
+            if (j < end1) {
+              wait(&bars.p_ready[1], np1++, kErrTensor);
+              if (!ok) break;
+              tc_fence_after();
+              values(1, ve, j == t0);
+              if (last == 1) umma_commit(&bars.kv_empty[ve % kStages]);
+              if (j + 1 < end1) begin(1);
+              else umma_commit(&bars.o_full[1]);
+            }
+            if (j + 2 == t1) umma_commit(&bars.q_empty);
+          }
+          tile0 += t1 - t0;
+        }
+        if (!ok) {
+          *failed = 1;
+          if (why) atomicOr(&g_attn_error, why);
+        }
+        umma_commit(&bars.drain);  // nothing is in flight when the block ends
+        mbar_wait(&bars.drain, 0);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int t = warp >> 2;        // tile of rows
+    const int r = tid & 127;        // row
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane field: 32 (warp % 4)
+    const uint32_t ts = tmem + 128 * t + lanes, to = tmem + 256 + 128 * t + lanes;
+    const int rtok = t * g.sub + r / grp;  // token of the block
+    uint32_t ns = 0, no = 0, tile0 = 0;
+    bool ok = true;
+    for (uint32_t n = 0;; ++n) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1));
+      const Work& w = sh.work[n % kWorks];
+      if (!ok || !w.live) break;
+      const bool mine = r < g.sub * grp && rtok < w.toks;
+      const int lim = mine ? max(w.lim0 + rtok, 0) : 0;  // keys that the row sees
+      const int kv_len = w.kv_len, t0 = w.t0, t1 = w.end[t];
+      float m = -INFINITY, l = 0.f;  // m in log2 units
+      for (int j = t0; j < t1; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], ns++ & 1));
+        if (!ok) break;
+        tc_fence_after();
+        float s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+        tmem_wait_ld();
+        const int vis = lim - j * kTile;  // visible columns of this tile
+        if (__any_sync(0xffffffffu, vis < kTile)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[c][i] = 32 * c + i < vis ? s[c][i] : -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, s[c][i]);
+        mx *= a.scale_log2;  // scale > 0
+        const bool raise = mx > m + kRaise;  // always for the first finite score
+        if (__any_sync(0xffffffffu, raise)) {
+          const float m2 = raise ? mx : m;
+          const float f = m == -INFINITY ? 0.f : ex2(m - m2);
+          l *= f;
+          if (j > t0) {  // O holds earlier tiles: their product is complete (s_full came after)
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {  // 16 columns at a time: few registers, rare
+              uint32_t o[16];
+              tmem_ld16(to + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(to + 16 * c, o);
+            }
+          }
+          m = m2;
+        }
+        const float mm = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = ex2(fmaf(s[c][2 * i], a.scale_log2, -mm));
+            const float y = ex2(fmaf(s[c][2 * i + 1], a.scale_log2, -mm));
+            sum += x + y;
+            pk[i] = pack_bf16(x, y);
+          }
+          tmem_st16(ts + 16 * c, pk);
+        }
+        l += sum;
+        if ((j + 1) * kTile > kv_len) {  // rows of V behind the last key
+          const uint32_t entry = 2 * (tile0 + j - t0) + 1;
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&bars.kv_full[entry % kStages], entry / kStages & 1));
+          if (ok && j * kTile + r >= kv_len) {
+            const uint32_t row = skv + entry % kStages * kTileBytes + r * 128;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              st_shared_v4(row + 16 * c, 0, 0, 0, 0);
+              st_shared_v4(row + kHalfBytes + 16 * c, 0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async();
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars.p_ready[t]);
+        if (!ok) break;
+      }
+      if (t1 > t0 && ok)
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[t], no++ & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const int slot = w.slot;
+      const bool saw = mine && lim > t0 * kTile;  // some key of the piece
+      if (slot < 0) {
+        const float inv = 1.f / l;
+        __nv_bfloat16* op = a.out + (w.row0 + rtok) * a.o_stride +
+                            ((long long)w.head * grp + r % grp) * kHeadDim;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          if (t1 > t0) {
+            tmem_ld32(to + 32 * c, o);
+            tmem_wait_ld();
+          }
+          if (mine) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                pk[k] = saw ? pack_bf16(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv) : 0u;
+              *reinterpret_cast<uint4*>(op + 32 * c + 8 * i) =
+                  make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          }
+        }
+      } else {
+        // a row that saw nothing of the piece: (-inf, 0), its sums are not read
+        float* part = attn_partial(p.ws, 2 * kRows, blockIdx.x, slot);
+        float* po = part + (long long)(t * kRows + r) * kHeadDim;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          if (t1 > t0) {
+            tmem_ld32(to + 32 * c, o);
+            tmem_wait_ld();
+          }
+          if (saw) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4*>(po + 32 * c + 4 * i) =
+                  make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
+        }
+        float* ml = part + (long long)2 * kRows * kHeadDim + 2 * (t * kRows + r);
+        ml[0] = saw ? m : -INFINITY;
+        ml[1] = saw ? l : 0.f;
+      }
+      tc_fence_before();
+      tile0 += w.t1 - t0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
+    }
+    if (!ok) {
+      *failed = 1;
+      if (lane == 0) atomicOr(&g_attn_error, kErrTensor);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
+}
+
+// [d2][d1][d0] bf16, strides in elements, boxes of 64 x b1 x b2 with the 128-byte swizzle.
+bool make_map(CUtensorMap* m, const void* base, long long d0, long long d1, long long d2,
+              long long s1, long long s2, int b1, int b2) {
+  auto fn = encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+  const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2}, one[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+unsigned read_attn_device_error(bool clear) {
+  unsigned v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attn_error, sizeof(v)) != cudaSuccess) return ~0u;
+  if (clear && v != 0) {
+    const unsigned zero = 0;
+    if (cudaMemcpyToSymbol(g_attn_error, &zero, sizeof(zero)) != cudaSuccess) return ~0u;
+  }
+  return v;
+}
+
+int attn_tc_rows() { return 2 * kRows; }
+
+cudaError_t launch_attn_tc(const AttnArgs& a, int sms, float* workspace, cudaStream_t st) {
+  const int grp = a.hq / a.hkv;
+  TcArgs p{};
+  p.a = a;
+  p.g.sub = kRows / grp;
+  p.g.block = 2 * p.g.sub;
+  p.g.sub_rows = kRows;
+  p.g.tile = kTile;
+  p.g.overhead = 128;
+  p.g.whole = 4;
+  p.ws = workspace;
+  CUtensorMap mq, mk, mv;
+  bool ok = make_map(&mq, a.q, kHeadDim, a.hq, a.total_q, kHeadDim, a.q_stride, grp, p.g.sub);
+  const long long kw = (long long)a.hkv * kHeadDim;
+  if (a.paged) {
+    int box = 128;
+    while (a.page_size % box != 0) box /= 2;
+    p.box = box;
+    ok = ok && make_map(&mk, a.k, kw, a.page_size, a.num_pages, kw, a.k_page_stride, box, 1) &&
+         make_map(&mv, a.v, kw, a.page_size, a.num_pages, kw, a.v_page_stride, box, 1);
+  } else {
+    p.box = 128;
+    ok = ok &&
+         make_map(&mk, a.k, kw, a.total_q, 1, a.k_stride, a.total_q * a.k_stride, 128, 1) &&
+         make_map(&mv, a.v, kw, a.total_q, 1, a.v_stride, a.total_q * a.v_stride, 128, 1);
+  }
+  if (!ok) return cudaErrorInvalidValue;
+  static thread_local int set_for = -1;  // the attribute belongs to the device's context
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (set_for != dev) {
+    e = cudaFuncSetAttribute(attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)kSmemBytes);
+    if (e != cudaSuccess) return e;
+    set_for = dev;
+  }
+  attn_tc_kernel<<<sms, kThreads, kSmemBytes, st>>>(mq, mk, mv, p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return launch_attn_join(a, p.g, 2 * kRows, sms, workspace, st);
+}
+
+}  // namespace gdn

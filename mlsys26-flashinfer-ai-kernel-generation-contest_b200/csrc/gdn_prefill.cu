@@ -225,8 +225,9 @@ extern "C" int gdn_device_error(int clear) {
   const unsigned d = gdn::read_decode_device_error(clear != 0);
   const unsigned e = gdn::read_segment_device_error(clear != 0);
   const unsigned t = gdn::read_selftest_device_error(clear != 0);
-  if (a == ~0u || b == ~0u || d == ~0u || e == ~0u || t == ~0u) return -1;
-  return (int)(a | b | d | e | t);
+  const unsigned x = gdn::read_attn_device_error(clear != 0);
+  if (a == ~0u || b == ~0u || d == ~0u || e == ~0u || t == ~0u || x == ~0u) return -1;
+  return (int)(a | b | d | e | t | x);
 }
 
 extern "C" int gdn_prefill_launch_strided(

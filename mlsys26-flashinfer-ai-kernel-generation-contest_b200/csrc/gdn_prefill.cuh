@@ -114,5 +114,7 @@ unsigned read_decode_device_error(bool clear);
 unsigned read_segment_device_error(bool clear);
 // Same for the bounded-wait self-test kernel (gdn_selftest_bounded_wait).
 unsigned read_selftest_device_error(bool clear);
+// Same for the attention kernels.
+unsigned read_attn_device_error(bool clear);
 
 }  // namespace gdn
