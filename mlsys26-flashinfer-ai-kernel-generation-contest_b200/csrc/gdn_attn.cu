@@ -1,6 +1,10 @@
 // C-ABI entry points of the softmax-attention operators: argument checks and the choice
 // of the kernel.
-#include <cmath>
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
+#include <chrono>
 
 #include "gdn_attn_sched.cuh"
 
@@ -23,38 +27,103 @@ bool bad_rows(const void* p, long long stride, long long width) {
 }
 
 // CTAs of a launch: one per SM of the current device (without one: what a size needs at most).
-constexpr int kMaxParts = 160;
 int parts() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0 ||
-      n > kMaxParts)
-    n = kMaxParts;
+      n > kAttnMaxParts)
+    n = kAttnMaxParts;
   return n;
 }
 
-size_t workspace_size() { return attn_partial_bytes(attn_tc_rows(), kMaxParts); }
+// Rows of an item for the few-rows kernel, or 0 where the tensor-core kernel runs.
+int few_rows(long long total_q, int num_seqs, int hq, int hkv) {
+  const long long rows = (total_q + num_seqs - 1) / num_seqs * (hq / hkv);
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 0;
+}
+
+size_t workspace_size(long long total_q, int num_seqs, int hq, int hkv) {
+  const int few = few_rows(total_q, num_seqs, hq, hkv);
+  return attn_workspace_bytes(few ? few : attn_tc_rows(), kAttnMaxParts);
+}
+
+// A launch's tag (48 bits, not 0), which memory that was not written by it holds by a chance
+// of 2^-48: a counter mixed by the finaliser of the splitmix64 generator.
+unsigned long long next_tag() {
+  static std::atomic<unsigned long long> count{
+      (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count()};
+  unsigned long long z = (count.fetch_add(1, std::memory_order_relaxed) + 1) * 0x9e3779b97f4a7c15ull;
+  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
+  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
+  z = (z ^ (z >> 31)) >> 16;
+  return z != 0 ? z : 1;
+}
 
 int launch(AttnArgs& p, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!workspace || workspace_bytes < workspace_size()) return GDN_ERR_WORKSPACE;
+  if (!workspace || workspace_bytes < workspace_size(p.total_q, p.num_seqs, p.hq, p.hkv))
+    return GDN_ERR_WORKSPACE;
   if (misaligned(workspace, 16)) return GDN_ERR_INVALID_ARGUMENT;
   p.scale_log2 = default_scale(scale) * 1.4426950408889634f;
-  return launch_attn_tc(p, parts(), static_cast<float*>(workspace),
-                        static_cast<cudaStream_t>(stream)) == cudaSuccess
-             ? GDN_OK
-             : GDN_ERR_LAUNCH;
+  const int few = few_rows(p.total_q, p.num_seqs, p.hq, p.hkv);
+  const unsigned long long tag = next_tag();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = few ? launch_attn_rows(p, few, parts(), workspace, tag, st)
+                            : launch_attn_tc(p, parts(), workspace, tag, st);
+  return e == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
 }
 
 }  // namespace
+
+bool attn_map(CUtensorMap* m, const void* base, long long d0, long long d1, long long d2,
+              long long s1, long long s2, int b1, int b2) {
+  auto fn = encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+  const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2}, one[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int attn_key_box(const AttnArgs& p, int most) {
+  int box = most;
+  while (p.paged && p.page_size % box != 0) box /= 2;
+  return box;
+}
+
+bool attn_key_maps(CUtensorMap* mk, CUtensorMap* mv, const AttnArgs& p, int box) {
+  const long long w = (long long)p.hkv * kHeadDim;
+  if (p.paged)
+    return attn_map(mk, p.k, w, p.page_size, p.num_pages, w, p.k_page_stride, box, 1) &&
+           attn_map(mv, p.v, w, p.page_size, p.num_pages, w, p.v_page_stride, box, 1);
+  return attn_map(mk, p.k, w, p.total_q, 1, p.k_stride, p.total_q * p.k_stride, box, 1) &&
+         attn_map(mv, p.v, w, p.total_q, 1, p.v_stride, p.total_q * p.v_stride, box, 1);
+}
+
+unsigned read_attn_device_error(bool clear) {
+  return read_attn_tc_error(clear) | read_attn_rows_error(clear);
+}
+
 }  // namespace gdn
 
 extern "C" size_t gdn_attn_workspace_size(int total_q, int num_seqs, int num_q_heads,
                                           int num_kv_heads) {
-  (void)total_q;
-  (void)num_seqs;
-  (void)num_q_heads;
-  (void)num_kv_heads;
-  return gdn::workspace_size();
+  if (total_q <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads) return 0;
+  return gdn::workspace_size(total_q, num_seqs, num_q_heads, num_kv_heads);
 }
 
 extern "C" int gdn_attn_prefill_launch(const void* q, const void* k, const void* v,

@@ -66,8 +66,24 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& p, int s) {
   return r;
 }
 
-// Tensor-core kernel on `sms` CTAs (workspace: attn_partial_bytes(attn_tc_rows(), sms)).
+// TMA maps: [d2][d1][d0] bf16, strides in elements, boxes of 64 x b1 x b2 with the 128-byte
+// swizzle; the maps of K and V (key rows of a page, or of the packed prompts), `box` rows high.
+bool attn_map(CUtensorMap* m, const void* base, long long d0, long long d1, long long d2,
+              long long s1, long long s2, int b1, int b2);
+bool attn_key_maps(CUtensorMap* mk, CUtensorMap* mv, const AttnArgs& p, int box);
+// The highest box (a power of two, at most `most`) that does not cross a page's end.
+int attn_key_box(const AttnArgs& p, int most);
+
+// Tensor-core kernel on `sms` CTAs (workspace: attn_workspace_bytes(attn_tc_rows(), sms));
+// `tag`: 48 bits, not 0, another one for every launch.
 int attn_tc_rows();
-cudaError_t launch_attn_tc(const AttnArgs& p, int sms, float* workspace, cudaStream_t st);
+cudaError_t launch_attn_tc(const AttnArgs& p, int sms, void* workspace, unsigned long long tag,
+                           cudaStream_t st);
+unsigned read_attn_tc_error(bool clear);
+
+// Kernel for few rows: an item has at most `rows` (16, 32 or 64) of them.
+cudaError_t launch_attn_rows(const AttnArgs& p, int rows, int sms, void* workspace,
+                             unsigned long long tag, cudaStream_t st);
+unsigned read_attn_rows_error(bool clear);
 
 }  // namespace gdn

@@ -1,0 +1,37 @@
+// Device pieces shared by the attention kernels.
+#pragma once
+
+#include "gdn_common.cuh"
+#include "sm100.cuh"
+
+namespace gdn {
+namespace sm100 {
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint64_t* bar,
+                                            int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+}  // namespace sm100
+
+// error bits of the kernels' bounded waits (gdn_device_error)
+constexpr unsigned kErrLoad = 1u, kErrTensor = 2u;
+
+// The maximum that a row's sums are relative to is raised only when it is exceeded by 2^8.
+constexpr float kRaise = 8.f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&b);
+}
+
+}  // namespace gdn

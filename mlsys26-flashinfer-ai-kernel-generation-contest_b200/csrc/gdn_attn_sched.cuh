@@ -18,12 +18,13 @@ namespace gdn {
 // a CTA has at most two partial pieces: of the item its range begins inside (slot 0) and
 // of the one its range ends inside (slot 1)
 constexpr int kAttnSlots = 2;
+constexpr int kAttnTile = 128;      // keys per tile
+constexpr int kAttnMaxParts = 160;  // CTAs that share the work (one per SM)
 
 struct AttnGrid {
   int block;     // query tokens per item
   int sub;       // query tokens per tile of rows: row (tok / sub) * sub_rows + (tok % sub) *
   int sub_rows;  // heads of the group + head
-  int tile;      // keys per tile
   int overhead;  // cost of an item's start and end, in keys
   int whole;     // items of at most this many tiles are not split
 };
@@ -58,7 +59,7 @@ __device__ __forceinline__ int attn_tile_at(const AttnGrid& g, int e, int n, lon
   if (x >= cost) return n;
   if (n <= g.whole) return 2 * x > cost ? n : 0;
   const long long y = x - g.overhead;
-  return y <= 0 ? 0 : (int)(y / g.tile);
+  return y <= 0 ? 0 : (int)((unsigned long long)y / kAttnTile);
 }
 
 struct AttnCursor {
@@ -108,87 +109,278 @@ struct AttnCursor {
   }
 };
 
-__device__ __forceinline__ long long attn_cut(long long total, int c, int parts) {
-  return total / parts * c + total % parts * c / parts;
-}
+// The line of all costs, cut into `parts`.
+struct AttnLine {
+  long long total, per;
+  int rest, parts;
+  __device__ __forceinline__ long long cut(int c) const {
+    return per * c + (unsigned)(rest * c) / (unsigned)parts;  // total * c / parts, rounded down
+  }
+};
 
-// The block's share of the line: range [u0, u1) and the sequence that u0 lies in.
+// What a CTA starts from: its range [u0, u1) and the sequence that u0 lies in.
 struct AttnShare {
-  long long total, u0, seq_start;
+  AttnLine line;
+  long long u0, u1, seq_start;
   int seq;
 };
 
-// Collective over a block of NT threads (a multiple of 32): the total cost, and the
-// sequence that holds the `c`-th of `parts` cuts.
+// Collective over a block of NT threads (a multiple of 32): the share of CTA c of `parts`.
 template <int NT>
 __device__ __forceinline__ void attn_share(const AttnArgs& p, const AttnGrid& g, int c, int parts,
                                            AttnShare* out) {
   __shared__ long long warp_sum[NT / 32];
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  long long mine = 0, own = 0;  // own: the cost of the last sequence looked at
-  for (int s = tid; s < p.num_seqs; s += NT) {
-    own = attn_head_cost(attn_seq(p, s), g) * p.hkv;
-    mine += own;
-  }
-  for (int w = 16; w > 0; w >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, w);
-  if (lane == 0) warp_sum[warp] = mine;
-  if (tid == 0) found = 0;
-  __syncthreads();
-  long long total = 0;
+  const bool one = p.num_seqs <= NT;  // a sequence a thread: one pass finds everything
+  long long mine = 0;
+  for (int s = tid; s < p.num_seqs; s += NT) mine += attn_head_cost(attn_seq(p, s), g) * p.hkv;
+  long long sum = mine;  // inclusive over the threads
 #pragma unroll
-  for (int w = 0; w < NT / 32; ++w) total += warp_sum[w];
-  const long long u = attn_cut(total, c, parts);
+  for (int w = 1; w < 32; w <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, sum, w);
+    if (lane >= w) sum += y;
+  }
+  if (lane == 31) warp_sum[warp] = sum;
+  __syncthreads();
+  AttnLine line;
+  line.total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w == warp) sum += line.total;
+    line.total += warp_sum[w];
+  }
+  line.per = line.total / parts;
+  line.rest = (int)(line.total - line.per * parts);
+  line.parts = parts;
+  const long long u = line.cut(c);
   if (tid == 0) {
-    out->total = total;
+    out->line = line;
     out->u0 = u;
-    out->seq = p.num_seqs;
-    out->seq_start = total;
+    out->u1 = line.cut(c + 1);
+    found = 0;
   }
-  __syncthreads();
-  long long base = 0;
-  for (int s0 = 0; s0 < p.num_seqs && u < total; s0 += NT) {
-    const int s = s0 + tid;
-    long long x = 0;
-    if (s < p.num_seqs)
-      x = p.num_seqs <= NT ? own : attn_head_cost(attn_seq(p, s), g) * p.hkv;
-    long long sum = x;
+  if (one) {
+    if (sum - mine <= u && u < sum) {
+      out->seq = tid;
+      out->seq_start = sum - mine;
+    }
+  } else {
+    long long base = 0;
+    for (int s0 = 0; s0 < p.num_seqs && u < line.total; s0 += NT) {
+      __syncthreads();
+      if (found) break;
+      const int s = s0 + tid;
+      const long long x = s < p.num_seqs ? attn_head_cost(attn_seq(p, s), g) * p.hkv : 0;
+      sum = x;
 #pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, sum, w);
-      if (lane >= w) sum += y;
-    }
-    if (lane == 31) warp_sum[warp] = sum;
-    __syncthreads();
-    long long all = 0;
+      for (int w = 1; w < 32; w <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, sum, w);
+        if (lane >= w) sum += y;
+      }
+      if (lane == 31) warp_sum[warp] = sum;
+      __syncthreads();
+      long long all = 0;
 #pragma unroll
-    for (int w = 0; w < NT / 32; ++w) {
-      if (w < warp) sum += warp_sum[w];
-      all += warp_sum[w];
+      for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) sum += warp_sum[w];
+        all += warp_sum[w];
+      }
+      sum += base;
+      if (x > 0 && sum - x <= u && u < sum) {
+        out->seq = s;
+        out->seq_start = sum - x;
+        found = 1;
+      }
+      base += all;
     }
-    sum += base;
-    if (x > 0 && sum - x <= u && u < sum) {
-      out->seq = s;
-      out->seq_start = sum - x;
-      found = 1;
-    }
-    base += all;
-    __syncthreads();
-    if (found) break;
   }
   __syncthreads();
 }
 
-// Partial results of a piece: rows of 128 fp32 sums, then (maximum in log2 units, sum) per row.
-__host__ __device__ inline size_t attn_partial_bytes(int rows, int parts) {
-  return (size_t)parts * kAttnSlots * rows * (kHeadDim + 2) * sizeof(float);
+// ---------------------------------------------------------------- partial results
+// Workspace: arrival counters, then for every CTA and slot the rows of 128 fp32 sums and
+// (maximum in log2 units, sum) of each row.
+constexpr int kAttnFan = 16;  // pieces that one CTA joins; more are joined in two levels
+struct AttnCounters {
+  unsigned long long arrived[kAttnMaxParts * kAttnSlots][2][2];  // [first piece][level][row tile]
+};
+__host__ __device__ inline size_t attn_workspace_bytes(int rows, int parts) {
+  return sizeof(AttnCounters) +
+         (size_t)parts * kAttnSlots * rows * (kHeadDim + 2) * sizeof(float);
 }
-__device__ __forceinline__ float* attn_partial(float* ws, int rows, int cta, int slot) {
-  return ws + ((long long)cta * kAttnSlots + slot) * rows * (kHeadDim + 2);
+struct AttnPartials {
+  AttnCounters* counters;
+  float* base;
+  unsigned long long tag;  // of this launch: 48 bits, not 0
+  int rows;
+  __device__ __forceinline__ float* sums(int piece) const {  // piece = 2 CTA + slot
+    return base + (long long)piece * rows * (kHeadDim + 2);
+  }
+  __device__ __forceinline__ float* stats(int piece) const {
+    return sums(piece) + (long long)rows * kHeadDim;
+  }
+};
+inline AttnPartials attn_partials(void* workspace, int rows, unsigned long long tag) {
+  return AttnPartials{static_cast<AttnCounters*>(workspace),
+                      reinterpret_cast<float*>(static_cast<AttnCounters*>(workspace) + 1), tag,
+                      rows};
+}
+// A counter's memory may hold anything before the first arrival: only a word with this
+// launch's tag counts.  The last of n arrivals (true) clears it, for the next replay of a
+// captured launch, whose tag is the same.
+__device__ __forceinline__ bool attn_arrive(unsigned long long* word, unsigned long long tag,
+                                            int n) {
+  unsigned long long seen = *static_cast<volatile unsigned long long*>(word);
+  while (true) {
+    const unsigned long long k = ((seen >> 16) == tag ? (seen & 0xffffu) : 0u) + 1;
+    const bool last = k == (unsigned long long)n;
+    const unsigned long long was = atomicCAS(word, seen, last ? 0ull : (tag << 16) | k);
+    if (was == seen) return last;
+    seen = was;
+  }
 }
 
-// Joins the pieces of split items (of `rows` rows); `parts` CTAs shared the work on `g`.
-cudaError_t launch_attn_join(const AttnArgs& p, const AttnGrid& g, int rows, int parts,
-                             float* workspace, cudaStream_t st);
+// The pieces of one item, in the order of the keys, as every one of its CTAs finds them.
+struct AttnPieces {
+  short list[kAttnMaxParts];  // 2 CTA + slot
+  int count, mine;            // mine: this CTA's place in the list
+};
+// By one warp, for the item `cur` (e keys, n tiles) and CTA `cta`.
+__device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& line,
+                                            long long start, int e, int n, int cta,
+                                            AttnPieces* out) {
+  const int lane = threadIdx.x & 31;
+  const long long end = start + e + g.overhead;
+  int count = 0;
+  for (int c0 = 0; c0 < line.parts; c0 += 32) {
+    const int c = c0 + lane;
+    bool has = false;
+    long long lo = 0;
+    if (c < line.parts) {
+      lo = line.cut(c);
+      const long long hi = line.cut(c + 1);
+      has = hi > start && lo < end &&
+            attn_tile_at(g, e, n, lo > start ? lo - start : 0) < attn_tile_at(g, e, n, hi - start);
+    }
+    const unsigned some = __ballot_sync(0xffffffffu, has);
+    if (has) {
+      const int at = count + __popc(some & ((1u << lane) - 1));
+      out->list[at] = (short)(2 * c + (lo > start ? 0 : 1));
+      if (c == cta) out->mine = at;
+    }
+    count += __popc(some);
+  }
+  if (lane == 0) out->count = count;
+}
+
+// Joins `count` <= kAttnFan pieces list[0], list[step], .. of the rows [row0, row0 + rows):
+// kWarps warps, R rows of each at a time (loads of all of them in flight).  Every row goes
+// to out(row, lane's four columns, maximum, sum).
+template <int kWarps, int R, typename Out>
+__device__ __forceinline__ void attn_merge(const AttnPartials& ws, const short* list, int step,
+                                           int count, int row0, int rows, int warp, Out&& out) {
+  constexpr int kPer = 32 / R, kRounds = kAttnFan / kPer;
+  const int lane = threadIdx.x & 31;
+  const int jl = lane / kPer, il = lane % kPer;  // the row and piece whose weight the lane has
+  for (int r = warp * R; r < rows; r += kWarps * R) {
+    float2 ml[kRounds];
+    float M = -INFINITY, l = 0.f, f[kRounds];
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int i = k * kPer + il;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (i < count && r + jl < rows)
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(ws.stats(list[i * step])) + row0 + r + jl);
+      if (ml[k].y != 0.f) M = fmaxf(M, ml[k].x);  // sum 0: the row saw nothing of the piece
+    }
+#pragma unroll
+    for (int w = 1; w < kPer; w <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      f[k] = ml[k].y == 0.f ? 0.f : exp2f(ml[k].x - M);
+      l += ml[k].y == 0.f ? 0.f : f[k] * ml[k].y;
+    }
+#pragma unroll
+    for (int w = 1; w < kPer; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    float4 o[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+#pragma unroll 2
+      for (int i = 0; i < kPer; ++i) {
+        if (k * kPer + i >= count) break;
+        const float* src = ws.sums(list[(k * kPer + i) * step]) +
+                           (long long)(row0 + r) * kHeadDim + 4 * lane;
+        float4 x[R];
+        float w[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          w[j] = __shfl_sync(0xffffffffu, f[k], j * kPer + i);
+          x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (w[j] != 0.f) x[j] = __ldcg(reinterpret_cast<const float4*>(src + j * kHeadDim));
+        }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          o[j].x = fmaf(w[j], x[j].x, o[j].x);
+          o[j].y = fmaf(w[j], x[j].y, o[j].y);
+          o[j].z = fmaf(w[j], x[j].z, o[j].z);
+          o[j].w = fmaf(w[j], x[j].w, o[j].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const float Mj = __shfl_sync(0xffffffffu, M, j * kPer);
+      const float lj = __shfl_sync(0xffffffffu, l, j * kPer);
+      if (r + j < rows) out(row0 + r + j, o[j], Mj, lj);
+    }
+  }
+}
+
+// After a piece's partial result is written: by the kWarps warps that wrote the rows [row0,
+// row0 + rows) (row tile `tile`) together, `sync` their barrier, `flag` an int of theirs in
+// shared memory.  The last CTA of an item to come here writes its output through
+// store(row, four columns).
+template <int kWarps, int R, typename Sync, typename Store>
+__device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPieces& pieces,
+                                          int tile, int row0, int rows, int warp, volatile int* flag,
+                                          Sync&& sync, Store&& store) {
+  const int lane = threadIdx.x & 31;
+  auto arrive = [&](int first, int level, int n) {  // true in the last CTA to arrive
+    __threadfence();
+    sync();
+    if (warp == 0 && lane == 0) {
+      *flag = attn_arrive(&ws.counters->arrived[pieces.list[first]][level][tile], ws.tag, n);
+      __threadfence();
+    }
+    sync();
+    return *flag != 0;
+  };
+  auto finish = [&](int row, float4 o, float, float l) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store(row, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+  };
+  const int n = pieces.count;
+  if (n <= kAttnFan) {
+    if (arrive(0, 0, n))
+      attn_merge<kWarps, R>(ws, pieces.list, 1, n, row0, rows, warp, finish);
+    return;
+  }
+  const int first = pieces.mine / kAttnFan * kAttnFan, some = min(kAttnFan, n - first);
+  if (!arrive(first, 0, some)) return;
+  const int head = pieces.list[first];  // the group's result replaces its first piece
+  attn_merge<kWarps, R>(ws, pieces.list + first, 1, some, row0, rows, warp,
+                        [&](int row, float4 o, float M, float l) {
+                          reinterpret_cast<float4*>(ws.sums(head) + (long long)row * kHeadDim)[lane] = o;
+                          __syncwarp();
+                          if (lane == 0)
+                            reinterpret_cast<float2*>(ws.stats(head))[row] = make_float2(M, l);
+                        });
+  const int groups = (n + kAttnFan - 1) / kAttnFan;
+  if (arrive(0, 1, groups))
+    attn_merge<kWarps, R>(ws, pieces.list, kAttnFan, groups, row0, rows, warp, finish);
+}
 
 }  // namespace gdn

@@ -18,12 +18,9 @@
 //
 // Key rows behind kv_len in a sequence's last tile can hold anything: their scores are
 // replaced, and their rows of V are zeroed in shared memory (0 * inf is not 0).
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
+#include "gdn_attn_dev.cuh"
 #include "gdn_attn_sched.cuh"
 #include "gdn_prefill.cuh"
-#include "sm100.cuh"
 
 namespace gdn {
 namespace {
@@ -31,17 +28,15 @@ namespace {
 using namespace sm100;
 
 constexpr int kRows = 128;             // rows of a tile
-constexpr int kTile = 128;             // keys of a tile
+constexpr int kTile = kAttnTile;       // keys of a tile
 constexpr int kStages = 5;             // K / V ring
 constexpr int kHalfBytes = 128 * 128;  // 64 columns of 128 rows, 128-byte swizzle
 constexpr int kTileBytes = 2 * kHalfBytes;
 constexpr int kThreads = 384;          // 168 registers a thread at launch: 64512
 // the softmax warps hold a row of scores: 256 x 216 + 128 x 72 registers = 64512
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
-constexpr float kRaise = 8.f;  // log2 of how far the maximum may be exceeded
 
 __device__ unsigned int g_attn_error = 0;
-constexpr unsigned kErrLoad = 1u, kErrTensor = 2u;
 
 constexpr int kWorks = 2;  // items handed out ahead
 struct Bars {
@@ -62,32 +57,38 @@ struct Work {
   int end[2];      // of which row tile 0 / 1 needs those below
   int slot;        // partial results' slot, -1: the piece is the whole item
   bool live;       // false: behind the last one
+  AttnPieces pieces;  // of the item, where it has more than this one
 };
 struct Shared {
   Bars bars;
   AttnShare share;
   Work work[kWorks];
   uint32_t tmem;
-  int failed;
+  int failed, joining[2];
 };
 constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + kStages * kTileBytes;
 
 struct TcArgs {
   AttnArgs a;
   AttnGrid g;
-  float* ws;
+  AttnPartials ws;
   int box;  // key rows per TMA box
 };
 
 // The piece of item `cur` inside [u0, u1); false if there is none.
-__device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& g, long long u0,
-                                         long long u1, Work* w) {
+// (By a whole warp; lane 0 writes it.)
+__device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& g,
+                                         const AttnShare& share, Work* w) {
+  const long long u0 = share.u0, u1 = share.u1;
   const int e = cur.keys(g);
   const int n = (e + kTile - 1) / kTile;
   const int t0 = attn_tile_at(g, e, n, u0 > cur.start ? u0 - cur.start : 0);
   const int t1 = attn_tile_at(g, e, n, u1 - cur.start);
   // an item without keys belongs to the CTA that it starts in (its rows are zeroed)
   if (t1 <= t0 && !(n == 0 && cur.start >= u0)) return false;
+  const int slot = (t0 == 0 && t1 == n) ? -1 : (u0 > cur.start ? 0 : 1);
+  if (slot >= 0) attn_pieces(g, share.line, cur.start, e, n, blockIdx.x, &w->pieces);
+  if ((threadIdx.x & 31) != 0) return true;
   const int first = cur.b * g.block;
   w->row0 = cur.seq.q0 + first;
   w->seq = cur.s;
@@ -104,18 +105,9 @@ __device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& 
     const int sees = toks > 0 ? w->lim0 + t * g.sub + toks - 1 : 0;
     w->end[t] = min(t1, sees > 0 ? (sees + kTile - 1) / kTile : 0);
   }
-  w->slot = (t0 == 0 && t1 == n) ? -1 : (u0 > cur.start ? 0 : 1);
+  w->slot = slot;
   w->live = true;
   return true;
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint64_t* bar,
-                                            int x, int y, int z) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-      : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -127,16 +119,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&b);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -152,7 +134,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const AttnGrid& g = p.g;
   const int grp = a.hq / a.hkv;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     Bars& b = sh.bars;
     for (int t = 0; t < 2; ++t) {
@@ -195,28 +176,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 10) {
       // ------------------------------------------------------------------ the pieces
-      if (lane == 0) {
-        const long long u0 = sh.share.u0;
-        const long long u1 = attn_cut(sh.share.total, blockIdx.x + 1, gridDim.x);
-        AttnCursor cur;
-        bool more = u0 < u1;
-        if (more) cur.seek(a, g, sh.share.seq, sh.share.seq_start, u0);
-        uint32_t n = 0;
-        bool ok = true;
-        while (ok) {
-          if (n >= kWorks) ok = mbar_wait(&bars.work_empty[n % kWorks], (n / kWorks - 1) & 1);
-          if (!ok || *failed) break;
-          Work* w = &sh.work[n % kWorks];
-          bool found = false;
-          while (more && !found) {
-            found = piece_of(cur, g, u0, u1, w);
-            more = cur.next(a, g) && cur.start < u1;
-          }
-          if (!found) w->live = false;
-          mbar_arrive(&bars.work_full[n % kWorks]);
-          if (!found) break;
-          ++n;
+      AttnCursor cur;
+      bool more = sh.share.u0 < sh.share.u1;
+      if (more) cur.seek(a, g, sh.share.seq, sh.share.seq_start, sh.share.u0);
+      for (uint32_t n = 0;; ++n) {
+        if (n >= kWorks && !__all_sync(0xffffffffu, mbar_wait(&bars.work_empty[n % kWorks],
+                                                              (n / kWorks - 1) & 1)))
+          break;
+        if (__any_sync(0xffffffffu, *failed)) break;
+        Work* w = &sh.work[n % kWorks];
+        bool found = false;
+        while (more && !found) {
+          found = piece_of(cur, g, sh.share, w);
+          more = cur.next(a, g) && cur.start < sh.share.u1;
         }
+        if (lane == 0 && !found) w->live = false;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.work_full[n % kWorks]);
+        if (!found) break;
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------------ loads
@@ -224,12 +201,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (uint32_t n = 0;; ++n) {
         ok = mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1);
-        const Work w = sh.work[n % kWorks];
-        __syncwarp();
-        if (!ok || !w.live || *failed) break;
-        if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
-        if (w.t1 <= w.t0) continue;
-        if (items > 0) ok = mbar_wait(&bars.q_empty, (items - 1) & 1);
+        const Work& w = sh.work[n % kWorks];  // handed back when its loads are issued
+        ok = __all_sync(0xffffffffu, ok && !*failed);
+        if (!ok || !w.live) break;
+        if (w.t1 <= w.t0) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
+          continue;
+        }
+        if (items > 0)
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_empty, (items - 1) & 1));
         if (!ok) break;
         if (lane == 0) {
           for (int t = 0; t < 2; ++t) {
@@ -275,12 +256,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
       }
       if (!ok) {
         *failed = 1;
         if (lane == 0) atomicOr(&g_attn_error, kErrLoad);
       }
-      if (!ok || *failed) {
+      if (!ok) {
         // copies in flight write into this block's memory: wait for them before it ends
         for (uint32_t i = ring > kStages ? ring - kStages : 0; i < ring; ++i)
           mbar_wait(&bars.kv_full[i % kStages], (i / kStages) & 1, 1u << 20);
@@ -394,8 +377,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (uint32_t n = 0;; ++n) {
       ok = __all_sync(0xffffffffu, mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1));
+      if (group_or(1 + t, 128, !ok)) {  // the four warps leave together
+        ok = false;
+        break;
+      }
       const Work& w = sh.work[n % kWorks];
-      if (!ok || !w.live) break;
+      if (!w.live) break;
       const bool mine = r < g.sub * grp && rtok < w.toks;
       const int lim = mine ? max(w.lim0 + rtok, 0) : 0;  // keys that the row sees
       const int kv_len = w.kv_len, t0 = w.t0, t1 = w.end[t];
@@ -475,7 +462,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (t1 > t0 && ok)
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[t], no++ & 1));
-      if (!ok) break;
+      if (group_or(1 + t, 128, !ok)) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
       const int slot = w.slot;
       const bool saw = mine && lim > t0 * kTile;  // some key of the piece
@@ -504,8 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         // a row that saw nothing of the piece: (-inf, 0), its sums are not read
-        float* part = attn_partial(p.ws, 2 * kRows, blockIdx.x, slot);
-        float* po = part + (long long)(t * kRows + r) * kHeadDim;
+        const int piece = 2 * blockIdx.x + slot;
+        float* po = p.ws.sums(piece) + (t * kRows + r) * kHeadDim;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float o[32];
@@ -520,9 +510,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                   make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
           }
         }
-        float* ml = part + (long long)2 * kRows * kHeadDim + 2 * (t * kRows + r);
-        ml[0] = saw ? m : -INFINITY;
-        ml[1] = saw ? l : 0.f;
+        reinterpret_cast<float2*>(p.ws.stats(piece))[t * kRows + r] =
+            saw ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        const int toks = min(w.toks - t * g.sub, g.sub);
+        if (toks > 0) {
+          const long long out0 = w.row0 + t * g.sub;
+          attn_join<4, 8>(
+              p.ws, w.pieces, t, t * kRows, toks * grp, warp & 3, &sh.joining[t],
+              [&] { group_sync(1 + t, 128); },
+              [&](int row, float4 x) {
+                const int i = row - t * kRows;
+                *reinterpret_cast<uint2*>(a.out + (out0 + i / grp) * a.o_stride +
+                                          ((long long)w.head * grp + i % grp) * kHeadDim +
+                                          4 * lane) =
+                    make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+              });
+        }
       }
       tc_fence_before();
       tile0 += w.t1 - t0;
@@ -541,35 +544,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 8) tmem_dealloc(tmem, 512);
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      ptr = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }();
-  return fn;
-}
-
-// [d2][d1][d0] bf16, strides in elements, boxes of 64 x b1 x b2 with the 128-byte swizzle.
-bool make_map(CUtensorMap* m, const void* base, long long d0, long long d1, long long d2,
-              long long s1, long long s2, int b1, int b2) {
-  auto fn = encoder();
-  if (!fn) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
-  const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2}, one[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 }  // namespace
 
-unsigned read_attn_device_error(bool clear) {
+unsigned read_attn_tc_error(bool clear) {
   unsigned v = 0;
   if (cudaMemcpyFromSymbol(&v, g_attn_error, sizeof(v)) != cudaSuccess) return ~0u;
   if (clear && v != 0) {
@@ -581,32 +558,21 @@ unsigned read_attn_device_error(bool clear) {
 
 int attn_tc_rows() { return 2 * kRows; }
 
-cudaError_t launch_attn_tc(const AttnArgs& a, int sms, float* workspace, cudaStream_t st) {
+cudaError_t launch_attn_tc(const AttnArgs& a, int sms, void* workspace, unsigned long long tag,
+                           cudaStream_t st) {
   const int grp = a.hq / a.hkv;
   TcArgs p{};
   p.a = a;
   p.g.sub = kRows / grp;
   p.g.block = 2 * p.g.sub;
   p.g.sub_rows = kRows;
-  p.g.tile = kTile;
   p.g.overhead = 128;
   p.g.whole = 4;
-  p.ws = workspace;
+  p.ws = attn_partials(workspace, 2 * kRows, tag);
   CUtensorMap mq, mk, mv;
-  bool ok = make_map(&mq, a.q, kHeadDim, a.hq, a.total_q, kHeadDim, a.q_stride, grp, p.g.sub);
-  const long long kw = (long long)a.hkv * kHeadDim;
-  if (a.paged) {
-    int box = 128;
-    while (a.page_size % box != 0) box /= 2;
-    p.box = box;
-    ok = ok && make_map(&mk, a.k, kw, a.page_size, a.num_pages, kw, a.k_page_stride, box, 1) &&
-         make_map(&mv, a.v, kw, a.page_size, a.num_pages, kw, a.v_page_stride, box, 1);
-  } else {
-    p.box = 128;
-    ok = ok &&
-         make_map(&mk, a.k, kw, a.total_q, 1, a.k_stride, a.total_q * a.k_stride, 128, 1) &&
-         make_map(&mv, a.v, kw, a.total_q, 1, a.v_stride, a.total_q * a.v_stride, 128, 1);
-  }
+  bool ok = attn_map(&mq, a.q, kHeadDim, a.hq, a.total_q, kHeadDim, a.q_stride, grp, p.g.sub);
+  p.box = attn_key_box(a, kTile);
+  ok = ok && attn_key_maps(&mk, &mv, a, p.box);
   if (!ok) return cudaErrorInvalidValue;
   static thread_local int set_for = -1;  // the attribute belongs to the device's context
   int dev = 0;
@@ -619,8 +585,7 @@ cudaError_t launch_attn_tc(const AttnArgs& a, int sms, float* workspace, cudaStr
     set_for = dev;
   }
   attn_tc_kernel<<<sms, kThreads, kSmemBytes, st>>>(mq, mk, mv, p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return launch_attn_join(a, p.g, 2 * kRows, sms, workspace, st);
+  return cudaGetLastError();
 }
 
 }  // namespace gdn
