@@ -149,19 +149,31 @@ def token_rows(x: torch.Tensor):
     return x.view(B * T, *x.shape[2:]) if B == 1 or x.stride(0) == T * x.stride(1) else None
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
 def on_device(device: torch.device):
-    """A context in which `device` is the current one (nothing is done if it is already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
+    """A context in which `device` is the current one."""
     return torch.cuda.device(device)
+
+
+class Plans(dict):
+    """Checked calls by their tensors' metadata (shape, strides, type, device; never their
+    addresses or values): what a call passes on besides its pointers.  A decode step costs a
+    few microseconds on the GPU, less than checking its arguments anew in Python."""
+    LIMIT = 4096
+
+    def keep(self, key, plan):
+        if len(self) >= self.LIMIT:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else \
+    torch.cuda.current_device
+
+
+def raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object
+    raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811

@@ -4,8 +4,9 @@
 ``cu_seqlens``); :func:`attn_paged` the form beside ``gdn_decode`` and ``gdn_mtp`` (one
 token, draft tokens or a chunk of a prompt per sequence, over a paged cache).  bf16, head
 size 128, grouped heads.  The lengths are read on the device only: no host synchronisation,
-and a captured graph follows them.  The work runs through the C ABI
-``gdn_attn_prefill_launch`` / ``gdn_attn_paged_launch``.
+and a captured graph follows them.  The work is one launch through the C ABI
+``gdn_attn_prefill_launch`` / ``gdn_attn_paged_launch``, with scratch from torch's caching
+allocator for each call, so that calls on several streams and captured graphs share none.
 """
 from __future__ import annotations
 
@@ -13,6 +14,8 @@ import torch
 
 from . import _checks as C
 from ._lib import LIB, check
+
+_prefill_plans, _paged_plans = C.Plans(), C.Plans()
 
 
 def _lengths(name, x, n, dev):
@@ -33,11 +36,23 @@ def _output(output, q, dev):
     return output
 
 
-def _workspace(dev, total_q, num_seqs, hq, hkv):
-    """(tensor, bytes): scratch of this call alone, from the caching allocator (so calls on
-    several streams and captured graphs never share it)."""
-    n = int(LIB.gdn_attn_workspace_size(total_q, num_seqs, hq, hkv))
-    return (torch.empty(n, dtype=torch.uint8, device=dev) if n else None), n
+def _workspace_bytes(total_q, num_seqs, hq, hk):
+    return int(LIB.gdn_attn_workspace_size(total_q, num_seqs, hq, hk))
+
+
+def _prefill_key(q, k, v, cu, out):
+    return (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
+            v.shape, v.stride(), v.dtype, v.device, cu.shape, cu.stride(), cu.dtype, cu.device,
+            out.shape, out.stride(), out.dtype, out.device)
+
+
+def _launch_prefill(plan, q, k, v, cu, sc, out):
+    ws_n, cu64, T, N, HQ, HK, qs, ks, vs, os_, dev = plan
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    status = LIB.gdn_attn_prefill_launch(q, k, v, cu, cu64, sc, out, T, N, HQ, HK, C.HEAD_SIZE, qs,
+                                         ks, vs, os_, ws.data_ptr(), ws_n, C.raw_stream(dev.index))
+    if status:
+        check("gdn_attn_prefill_launch", status)
 
 
 def attn_prefill(q, k, v, cu_seqlens, scale=None, output=None):
@@ -52,6 +67,22 @@ def attn_prefill(q, k, v, cu_seqlens, scale=None, output=None):
     A token's output does not depend on other sequences, nor, for finite values, on later
     tokens (a later value that is infinite or NaN can reach the earlier rows of its tile, as
     0 * inf)."""
+    try:
+        out = torch.empty_like(q) if output is None else output
+        plan = _prefill_plans.get(_prefill_key(q, k, v, cu_seqlens, out))
+    except (AttributeError, TypeError):
+        plan = None
+    if plan is not None and C.current_device() == plan[-1].index:
+        qp, kp, vp, op = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        cp = cu_seqlens.data_ptr()
+        if not (qp | kp | vp | op) & 15 and not cp & 7:
+            _launch_prefill(plan, qp, kp, vp, cp, C.scale_arg(scale), op)
+            return out
+    return _prefill_checked(q, k, v, cu_seqlens, scale, output)
+
+
+def _prefill_checked(q, k, v, cu_seqlens, scale, output):
+    """Every check; layouts that the kernels do not take are copied."""
     dev = C.cuda_device(q)
     C.tensor("q", q, torch.bfloat16, 3, dev, strided=True)
     C.tensor("k", k, torch.bfloat16, 3, dev, strided=True)
@@ -68,18 +99,38 @@ def attn_prefill(q, k, v, cu_seqlens, scale=None, output=None):
     if T == 0 or N == 0:
         return output
     with C.on_device(dev):
-        (q, qs), (k, ks), (v, vs) = C.rows_in(q, 8, 16), C.rows_in(k, 8, 16), C.rows_in(v, 8, 16)
+        cu = C.dense_or_copy(cu_seqlens, 8)
+        (x, qs), (y, ks), (z, vs) = C.rows_in(q, 8, 16), C.rows_in(k, 8, 16), C.rows_in(v, 8, 16)
         out, os_, back = C.rows_out(output, 8, 16)
         if back:
             out.copy_(output)  # rows behind the last sequence keep their values
-        ws, ws_n = _workspace(dev, T, N, HQ, HK)
-        check("gdn_attn_prefill_launch", LIB.gdn_attn_prefill_launch(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(),
-            cu_seqlens.dtype == torch.int64, sc, out.data_ptr(), T, N, HQ, HK, D, qs, ks, vs, os_,
-            ws.data_ptr() if ws is not None else None, ws_n, C.stream_handle(dev)))
+        plan = (_workspace_bytes(T, N, HQ, HK), int(cu.dtype == torch.int64), T, N, HQ, HK, qs, ks,
+                vs, os_, torch.device("cuda", q.get_device()))
+        _launch_prefill(plan, x.data_ptr(), y.data_ptr(), z.data_ptr(), cu.data_ptr(), sc,
+                        out.data_ptr())
         if back:
             output.copy_(out)
+        elif x is q and y is k and z is v:
+            _prefill_plans.keep(_prefill_key(q, k, v, cu_seqlens, output), plan)
     return output
+
+
+def _paged_key(q, k, v, table, lens, cu, out):
+    return (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
+            v.shape, v.stride(), v.dtype, v.device, table.shape, table.stride(), table.dtype,
+            table.device, lens.shape, lens.stride(), lens.dtype, lens.device, out.shape,
+            out.stride(), out.dtype, out.device,
+            None if cu is None else (cu.shape, cu.stride(), cu.dtype, cu.device))
+
+
+def _launch_paged(plan, q, k, v, table, lens, cu, sc, out):
+    (ws_n, ts, lens64, cu64, T, N, width, pages, page_size, kps, vps, HQ, HK, qs, os_, dev) = plan
+    ws = torch.empty(ws_n, dtype=torch.uint8, device=dev)
+    status = LIB.gdn_attn_paged_launch(q, k, v, table, ts, lens, lens64, cu, cu64, sc, out, T, N,
+                                       width, pages, page_size, kps, vps, HQ, HK, C.HEAD_SIZE, qs,
+                                       os_, ws.data_ptr(), ws_n, C.raw_stream(dev.index))
+    if status:
+        check("gdn_attn_paged_launch", status)
 
 
 def attn_paged(q, k_cache, v_cache, block_table, kv_lens, scale=None, output=None, *,
@@ -99,6 +150,24 @@ def attn_paged(q, k_cache, v_cache, block_table, kv_lens, scale=None, output=Non
     width * page_size counts as that.  What lies behind kv_len in a page is not used,
     whatever it holds; as in :func:`attn_prefill`, a newer token's infinite or NaN value can
     reach older rows of its tile."""
+    try:
+        out = torch.empty_like(q) if output is None else output
+        plan = _paged_plans.get(_paged_key(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens,
+                                           out))
+    except (AttributeError, TypeError):
+        plan = None
+    if plan is not None and C.current_device() == plan[-1].index:
+        qp, kp, vp, op = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+        tp, lp = block_table.data_ptr(), kv_lens.data_ptr()
+        cp = None if cu_seqlens is None else cu_seqlens.data_ptr()
+        if not (qp | kp | vp | op) & 15:
+            _launch_paged(plan, qp, kp, vp, tp, lp, cp, C.scale_arg(scale), op)
+            return out
+    return _paged_checked(q, k_cache, v_cache, block_table, kv_lens, scale, output, cu_seqlens)
+
+
+def _paged_checked(q, k_cache, v_cache, block_table, kv_lens, scale, output, cu_seqlens):
+    """Every check; layouts of q and output that the kernels do not take are copied."""
     dev = C.cuda_device(q)
     packed = cu_seqlens is not None
     C.tensor("q", q, torch.bfloat16, 3 if packed else 4, dev, strided=True)
@@ -131,28 +200,26 @@ def attn_paged(q, k_cache, v_cache, block_table, kv_lens, scale=None, output=Non
     if T == 0 or N == 0:
         return output
     with C.on_device(dev):
-        x, out, back = q, output, False
-        if not packed:  # rows of one token: [N, q_len, HQ, D] -> [T, HQ, D]
-            x, out = C.token_rows(q), C.token_rows(output)
-            if out is None:
-                out, back = torch.empty((T, HQ, D), dtype=torch.bfloat16, device=dev), True
-            if x is None:
-                x = q.reshape(T, HQ, D)
-        x, qs = C.rows_in(x, 8, 16)
+        x, out = (q, output) if packed else (C.token_rows(q), C.token_rows(output))
+        rows = x  # None: q's tokens are not one stride apart
+        x, qs = C.rows_in(q.reshape(T, HQ, D) if x is None else x, 8, 16)
+        back = out is None
         if not back:
             out, os_, back = C.rows_out(out, 8, 16)
         else:
-            os_ = HQ * D
+            out, os_ = torch.empty((T, HQ, D), dtype=torch.bfloat16, device=dev), HQ * D
         if back:
             out.copy_(output.reshape(T, HQ, D))  # rows behind the last sequence stay
-        ws, ws_n = _workspace(dev, T, N, HQ, HK)
-        check("gdn_attn_paged_launch", LIB.gdn_attn_paged_launch(
-            x.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-            block_table.stride(0) if N > 1 else width, kv_lens.data_ptr(),
-            kv_lens.dtype == torch.int64, cu_seqlens.data_ptr() if packed else None,
-            packed and cu_seqlens.dtype == torch.int64, sc, out.data_ptr(), T, N, width, pages,
-            page_size, kps, vps, HQ, HK, D, qs, os_, ws.data_ptr() if ws is not None else None,
-            ws_n, C.stream_handle(dev)))
+        plan = (_workspace_bytes(T, N, HQ, HK), block_table.stride(0) if N > 1 else width,
+                int(kv_lens.dtype == torch.int64),
+                int(packed and cu_seqlens.dtype == torch.int64), T, N, width, pages, page_size, kps,
+                vps, HQ, HK, qs, os_, torch.device("cuda", q.get_device()))
+        _launch_paged(plan, x.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                      block_table.data_ptr(), kv_lens.data_ptr(),
+                      cu_seqlens.data_ptr() if packed else None, sc, out.data_ptr())
         if back:
             output.copy_(out.view(output.shape))
+        elif x is rows:
+            _paged_plans.keep(_paged_key(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens,
+                                         output), plan)
     return output

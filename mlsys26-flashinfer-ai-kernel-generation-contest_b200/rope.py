@@ -18,6 +18,8 @@ from ._lib import LIB, check
 
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
+_plans = C.Plans()
+
 
 def rope_table(max_position: int, rotary_dim: int, *, base: float = 10000.0,
                scaling: str = "none", factor: float = 1.0, original_max_position: int = 0,
@@ -82,8 +84,63 @@ def _weight(name, w, dev):
     return C.dense_or_copy(w, 16)
 
 
-def _launch(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight, q_out, k_out,
-            eps, interleaved):
+def _key(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight, q_out, k_out):
+    return (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device,
+            positions.shape, positions.stride(), positions.dtype, positions.device, table.shape,
+            table.stride(), table.dtype, table.device, q_out.shape, q_out.stride(), q_out.dtype,
+            q_out.device,
+            None if q_weight is None else (q_weight.shape, q_weight.stride(), q_weight.dtype,
+                                           q_weight.device),
+            None if k_weight is None else (k_weight.shape, k_weight.stride(), k_weight.dtype,
+                                           k_weight.device),
+            (k_out.shape, k_out.stride(), k_out.dtype, k_out.device) if k_cache is None else
+            (v.shape, v.stride(), v.dtype, v.device, slots.shape, slots.stride(), slots.dtype,
+             slots.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device,
+             v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device))
+
+
+def _launch(plan, ptrs, eps, interleaved):
+    (pos64, rows, slots64, pages, page_size, kps, vps, T, HQ, HK, rd, qs, ks, vs, qos, kos,
+     dev) = plan
+    q, k, v, pos, table, wq, wk, qo, ko, slots, kc, vc = ptrs
+    status = LIB.gdn_attn_qk_norm_rope_launch(
+        q, k, v, pos, pos64, table, rows, wq, wk, eps, interleaved, qo, ko, slots, slots64, kc, vc,
+        pages, page_size, kps, vps, T, HQ, HK, C.HEAD_SIZE, rd, qs, ks, vs, qos, kos,
+        C.raw_stream(dev.index))
+    if status:
+        check("gdn_attn_qk_norm_rope_launch", status)
+
+
+def _run(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight, q_out, k_out, eps,
+         interleaved):
+    try:
+        qo = torch.empty_like(q) if q_out is None else q_out
+        ko = torch.empty_like(k) if k_out is None and k_cache is None else k_out
+        plan = _plans.get(_key(q, k, v, positions, table, slots, k_cache, v_cache, q_weight,
+                               k_weight, qo, ko))
+    except (AttributeError, TypeError):
+        plan = None
+    if plan is not None and C.current_device() == plan[-1].index and 0.0 <= eps < math.inf:
+        qp, kp, op = q.data_ptr(), k.data_ptr(), qo.data_ptr()
+        wq = 0 if q_weight is None else q_weight.data_ptr()
+        wk = 0 if k_weight is None else k_weight.data_ptr()
+        if k_cache is None:
+            vp = sp = kcp = vcp = None
+            bits = kop = ko.data_ptr()
+        else:
+            vp, kcp, vcp = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+            kop, sp, bits = None, slots.data_ptr(), vp | kcp | vcp
+        if not (qp | kp | op | wq | wk | bits) & 15:
+            _launch(plan, (qp, kp, vp, positions.data_ptr(), table.data_ptr(), wq or None,
+                           wk or None, op, kop, sp, kcp, vcp), eps, 1 if interleaved else 0)
+            return qo, ko
+    return _run_checked(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight,
+                        q_out, k_out, eps, interleaved)
+
+
+def _run_checked(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight, q_out,
+                 k_out, eps, interleaved):
+    """Every check; layouts that the kernel does not take are copied."""
     dev = C.cuda_device(q)
     C.tensor("q", q, torch.bfloat16, 3, dev, strided=True)
     C.tensor("k", k, torch.bfloat16, 3, dev, strided=True)
@@ -96,17 +153,18 @@ def _launch(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weig
     rd = table.shape[1]
     if rd < 2 or rd > D or rd % 2:
         raise ValueError(f"rope_table must have an even 2..{D} columns, got {rd}")
-    q_weight, k_weight = _weight("q_weight", q_weight, dev), _weight("k_weight", k_weight, dev)
     eps = float(eps)
     if not (0.0 <= eps < math.inf):
         raise ValueError(f"eps must be >= 0 and finite, got {eps}")
+    given = (q, k, v, q_weight, k_weight)
     if q_out is None:
         q_out = torch.empty(T, HQ, D, dtype=torch.bfloat16, device=dev)
     else:
         C.tensor("q_out", q_out, torch.bfloat16, 3, dev, strided=True)
         C.shape("q_out", q_out, (T, HQ, D))
     cached = k_cache is not None
-    kps = vps = pages = page_size = 0
+    kps = vps = pages = vs = kos = 0
+    page_size = 1
     if cached:
         C.tensor("v", v, torch.bfloat16, 3, dev, strided=True)
         C.shape("v", v, (T, HK, D))
@@ -118,33 +176,32 @@ def _launch(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weig
     else:
         C.tensor("k_out", k_out, torch.bfloat16, 3, dev, strided=True)
         C.shape("k_out", k_out, (T, HK, D))
-    if T == 0:
-        return q_out, k_out
-    q, qs = C.rows_in(q, 8, 16)
-    k, ks = C.rows_in(k, 8, 16)
-    vp = vs = kop = kos = 0
-    k_back = False
-    if cached:
-        v, vs = C.rows_in(v, 8, 16)
-        vp = v.data_ptr()
-    else:
-        ko, kos, k_back = C.rows_out(k_out, 8, 16)
-        kop = ko.data_ptr()
-    qo, qos, q_back = C.rows_out(q_out, 8, 16)
     with C.on_device(dev):
-        check("gdn_attn_qk_norm_rope_launch", LIB.gdn_attn_qk_norm_rope_launch(
-            q.data_ptr(), k.data_ptr(), vp or None, positions.data_ptr(),
-            positions.dtype == torch.int64, table.data_ptr(), table.shape[0],
-            q_weight.data_ptr() if q_weight is not None else None,
-            k_weight.data_ptr() if k_weight is not None else None, eps, bool(interleaved),
-            qo.data_ptr(), kop or None, slots.data_ptr() if cached else None,
-            cached and slots.dtype == torch.int64, k_cache.data_ptr() if cached else None,
-            v_cache.data_ptr() if cached else None, pages, page_size, kps, vps, T, HQ, HK, D, rd,
-            qs, ks, vs, qos, kos, C.stream_handle(dev)))
+        wq, wk = _weight("q_weight", q_weight, dev), _weight("k_weight", k_weight, dev)
+        if T == 0:
+            return q_out, k_out
+        x, qs = C.rows_in(q, 8, 16)
+        y, ks = C.rows_in(k, 8, 16)
+        z, ko, k_back = v, None, False
+        if cached:
+            z, vs = C.rows_in(v, 8, 16)
+        else:
+            ko, kos, k_back = C.rows_out(k_out, 8, 16)
+        qo, qos, q_back = C.rows_out(q_out, 8, 16)
+        plan = (int(positions.dtype == torch.int64), table.shape[0],
+                int(cached and slots.dtype == torch.int64), pages, page_size, kps, vps, T, HQ, HK,
+                rd, qs, ks, vs, qos, kos, torch.device("cuda", q.get_device()))
+        ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        _launch(plan, (ptr(x), ptr(y), ptr(z) if cached else None, ptr(positions), ptr(table),
+                       ptr(wq), ptr(wk), ptr(qo), ptr(ko), ptr(slots) if cached else None,
+                       ptr(k_cache), ptr(v_cache)), eps, int(bool(interleaved)))
         if q_back:
             q_out.copy_(qo)
         if k_back:
             k_out.copy_(ko)
+    if not q_back and not k_back and all(a is b for a, b in zip((x, y, z, wq, wk), given)):
+        _plans.keep(_key(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight,
+                         q_out, k_out), plan)
     return q_out, k_out
 
 
@@ -158,8 +215,8 @@ def attn_qk_norm_rope(q, k, positions, rope_table, q_weight=None, k_weight=None,
     ``interleaved``, (2i, 2i + 1).  A token whose position lies outside the table is padding:
     zeros.  Inputs and outputs may be views whose token rows are strided; other layouts go
     through dense temporaries."""
-    return _launch(q, k, None, positions, rope_table, None, None, None, q_weight, k_weight, q_out,
-                   k_out, eps, interleaved)
+    return _run(q, k, None, positions, rope_table, None, None, None, q_weight, k_weight, q_out,
+                k_out, eps, interleaved)
 
 
 def attn_append(q, k, v, positions, rope_table, slots, k_cache, v_cache, q_weight=None,
@@ -173,5 +230,5 @@ def attn_append(q, k, v, positions, rope_table, slots, k_cache, v_cache, q_weigh
     position lies outside the table is padding: zeros in q_out, nothing in the cache."""
     if k_cache is None:
         raise TypeError("k_cache must be a torch.Tensor, got NoneType")
-    return _launch(q, k, v, positions, rope_table, slots, k_cache, v_cache, q_weight, k_weight,
-                   q_out, None, eps, interleaved)[0]
+    return _run(q, k, v, positions, rope_table, slots, k_cache, v_cache, q_weight, k_weight, q_out,
+                None, eps, interleaved)[0]
