@@ -4,11 +4,12 @@
 // An item has up to R = 16, 32 or 64 rows: the query heads of one key/value head for as
 // many tokens as fit.  Every SM runs one CTA whose eight consumer warps split the keys:
 // with R = 16 MT, MT warps (16 rows each) share a chunk of 16 MT keys and there are 8 / MT
-// such groups, each with a ring of three chunks in shared memory (192 KB in all, what keeps
-// about 28 MB of loads in flight over the card) that one loader warp fills by TMA, a lane
-// per group.  16 rows per mma.sync m16n8k16: the tensor work is 2 % of the time that the
-// keys take to arrive, and a 128-row tcgen05 tile would be mostly padding and a longer chain
-// (it measured 378 us for 128 sequences of up to 8192 tokens).
+// such groups.  Each group keeps a ring of three chunks in shared memory that its own lanes
+// fill by cp.async, two chunks ahead, across the ends of pieces (192 KB a CTA, 128 KB of them
+// in flight); a box of 16 keys is too small for TMA, whose issue then bounds the loads (2 KB
+// boxes measured 5.2 TB/s from eight lanes and 2.0 TB/s from one).  16 rows per mma.sync
+// m16n8k16: the tensor work is a few per cent of the time that the keys take to arrive, and a
+// 128-row tcgen05 tile would be mostly padding and a longer chain.
 //
 // Each warp keeps its own running maximum, sum and output in registers (raised lazily, as in
 // the tensor-core kernel); the groups are joined through shared memory at the end of a piece,
@@ -22,12 +23,15 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kWarps = 8;    // consumers
-constexpr int kRing = 3;     // chunks per group
-constexpr int kTile = kAttnTile;  // keys that all groups take together
-constexpr int kWorks = 2;
-constexpr int kThreads = (kWarps + 2) * 32;
-constexpr size_t kSmemBytes = 1024 + (size_t)kRing * kTile * 2 * kHeadDim * 2;
+constexpr int kWarps = 12;   // consumers
+constexpr int kRing = 2;     // chunks per group
+constexpr int kTile = kAttnTile;
+constexpr int kRound = 16 * kWarps;  // keys that all groups take together
+constexpr int kWorks = 4;   // pieces handed out ahead
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr size_t smem_bytes(int rows) {  // ring, queries
+  return 1024 + (size_t)kRing * kRound * 2 * kHeadDim * 2 + (size_t)rows * kHeadDim * 2;
+}
 
 __device__ unsigned int g_rows_error = 0;
 
@@ -35,7 +39,6 @@ struct RowsArgs {
   AttnArgs a;
   AttnGrid g;
   AttnPartials ws;
-  int box;
 };
 struct Work {
   long long row0;   // query row of the block's first token
@@ -62,8 +65,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4])
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
       "{%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -71,8 +73,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 template <int MT>
 __global__ void __launch_bounds__(kThreads, 1)
-    attn_rows_kernel(const __grid_constant__ CUtensorMap mk,
-                     const __grid_constant__ CUtensorMap mv, const RowsArgs p) {
+    attn_rows_kernel(const __grid_constant__ RowsArgs p) {
   constexpr int kGroups = kWarps / MT;
   constexpr int kChunk = 16 * MT;              // keys
   constexpr int kHalf = kChunk * 128;          // 64 columns of a chunk's K or V
@@ -80,7 +81,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kRowsItem = 16 * MT;
   static_assert(kRowsItem * kHeadDim * 4 == kStage, "the join goes through a stage");
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[kGroups][kRing], empty[kGroups][kRing];
   __shared__ uint64_t work_full[kWorks], work_empty[kWorks];
   __shared__ Work works[kWorks];
   __shared__ AttnShare share;
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t kept[kGroups];           // the stage that holds a group's output
   __shared__ int failed_flag, joining;
   const uint32_t ring0 = smem_u32(raw) + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t sq = ring0 + kRing * kRound * 2 * kHeadDim * 2;  // the item's queries
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttnArgs& a = p.a;
   const AttnGrid& g = p.g;
@@ -95,23 +96,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* failed = &failed_flag;
 
   if (tid == 0) {
-    for (int i = 0; i < kGroups; ++i)
-      for (int j = 0; j < kRing; ++j) {
-        mbar_init(&full[i][j], 1);
-        mbar_init(&empty[i][j], MT);
-      }
     for (int i = 0; i < kWorks; ++i) {
       mbar_init(&work_full[i], 1);
-      mbar_init(&work_empty[i], 1 + kWarps);
+      mbar_init(&work_empty[i], kWarps);
     }
     fence_mbar_init();
     failed_flag = 0;
-    tma_prefetch_desc(&mk);
-    tma_prefetch_desc(&mv);
   }
   attn_share<kThreads>(a, g, blockIdx.x, gridDim.x, &share);  // ends with __syncthreads
 
-  if (warp == kWarps + 1) {
+  if (warp == kWarps) {
     // ------------------------------------------------------------------ the pieces
     const long long u0 = share.u0, u1 = share.u1;
     AttnCursor cur;
@@ -154,119 +148,153 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&work_full[n % kWorks]);
       if (!found) break;
     }
-  } else if (warp == kWarps) {
-    // ------------------------------------------------------------------ loads
-    uint32_t done = 0;  // chunks of this lane's group
-    bool ok = true;
-    for (uint32_t n = 0;; ++n) {
-      ok = mbar_wait(&work_full[n % kWorks], n / kWorks & 1);
-      const Work& w = works[n % kWorks];  // handed back when its loads are issued
-      ok = __all_sync(0xffffffffu, ok && !*failed);
-      if (!ok || !w.live) break;
-      const int* table = a.paged ? a.block_table + w.seq * a.table_stride : nullptr;
-      const int x = w.head * kHeadDim;
-      if (lane < kGroups) {
-        for (int key0 = w.k0 + lane * kChunk; key0 < w.k1; key0 += kTile) {
-          const uint32_t st = done % kRing;
-          if (done >= kRing) ok = mbar_wait(&empty[lane][st], (done / kRing - 1) & 1);
-          ok = ok && !*failed;
-          if (!ok) break;
-          mbar_arrive_expect_tx(&full[lane][st], kStage);
-          const uint32_t dst = ring0 + (lane * kRing + st) * kStage;
-          for (int i = 0; i < kChunk; i += p.box) {
-            const int key = key0 + i;
-            int row, page;
-            if (table == nullptr) {
-              row = w.kv0 + key;
-              page = 0;
-            } else {
-              row = key % a.page_size;
-              page = key < w.kv_len ? __ldg(table + key / a.page_size) : -1;  // -1: not used
-              if (page < 0 || page >= a.num_pages) page = -1;  // no such page: zeros
-            }
-            for (int h = 0; h < 2; ++h) {
-              tma_load_3d(dst + h * kHalf + i * 128, &mk, &full[lane][st], x + 64 * h, row, page);
-              tma_load_3d(dst + (2 + h) * kHalf + i * 128, &mv, &full[lane][st], x + 64 * h, row,
-                          page);
-            }
-          }
-          ++done;
-        }
-      }
-      __syncwarp();
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive(&work_empty[n % kWorks]);
-    }
-    if (!ok) {
-      *failed = 1;
-      if (lane == 0) atomicOr(&g_rows_error, kErrLoad);
-    }
-    if (!ok && lane < kGroups) {
-      // copies in flight write into this block's memory: wait for them before it ends
-      for (uint32_t i = done > kRing ? done - kRing : 0; i < done; ++i)
-        mbar_wait(&full[lane][i % kRing], i / kRing & 1, 1u << 20);
-    }
   } else {
     // ------------------------------------------------------------------ consumers
     const int group = warp / MT;
     const int mrow = (warp % MT) * 16;             // first row of the warp's tile
     const int qr = lane >> 2, qc = lane & 3;       // rows qr, qr + 8; column pair of a fragment
-    uint32_t done = 0;
+    const uint32_t stages = ring0 + group * kRing * kStage;
+    uint32_t done = 0;  // chunks consumed
     bool ok = true;
+
+    // The loads run ahead of the pieces, up to the last one handed out.  Lane l < 16 knows the
+    // page of key l of the warp's 16 in the next chunk, lane 16 + l too (the first half makes
+    // K's addresses, the other V's).
+    uint32_t issued = 0, ln = 0;
+    bool opened = false, more = true;  // piece ln has a next chunk; pieces left
+    int lkey = 0, lk1 = 0, lend = 0, lkv0 = 0, page = 0;
+    int lrow = 0, lidx = 0;  // of the lane's key: row of its page, place of the page in the table
+    const int* ltable = nullptr;
+    const __nv_bfloat16* lbase = nullptr;
+    const long long page_stride = !a.paged ? 0 : lane < 16 ? a.k_page_stride : a.v_page_stride;
+    const long long row_stride = a.paged ? (long long)a.hkv * kHeadDim
+                                         : (lane < 16 ? a.k_stride : a.v_stride);
+    const int step_pages = a.paged ? kRound / a.page_size : 0;
+    const int step_rows = kRound - step_pages * (a.paged ? a.page_size : 0);
+    auto find_page = [&] {  // asked for a chunk ahead of its use
+      if (a.paged) page = lkey + mrow + (lane & 15) < lend ? __ldg(ltable + lidx) : -1;
+    };
+    // To the next chunk; `n` is the piece at hand (a wait for one kWorks later would not end).
+    auto open = [&](uint32_t n) {
+      while (!opened && more && ln < n + kWorks) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&work_full[ln % kWorks], ln / kWorks & 1))) {
+          ok = more = false;
+          break;
+        }
+        const Work& w = works[ln % kWorks];
+        more = w.live;
+        lkey = w.k0 + group * kChunk;
+        lk1 = w.k1;
+        if (more && lkey < lk1) {
+          opened = true;
+          lend = w.kv_len;
+          lkv0 = w.kv0;
+          const int key = lkey + mrow + (lane & 15);
+          lidx = a.paged ? key / a.page_size : 0;
+          lrow = a.paged ? key - lidx * a.page_size : lkv0 + key;
+          lbase = (lane < 16 ? a.k : a.v) + (long long)w.head * kHeadDim;
+          ltable = a.paged ? a.block_table + w.seq * a.table_stride : nullptr;
+          find_page();
+        } else {
+          ++ln;
+        }
+      }
+      return opened;
+    };
+    auto issue = [&] {  // its loads: keys behind the last one and missing pages become zeros
+      const bool there = lkey + mrow + (lane & 15) < lend &&
+                         (!a.paged || (page >= 0 && page < a.num_pages));
+      const unsigned long long from = reinterpret_cast<unsigned long long>(
+          there ? lbase + page * page_stride + lrow * row_stride : a.k);
+      const uint32_t valid = __ballot_sync(0xffffffffu, there);
+      const uint32_t dst = stages + issued % kRing * kStage;
+      const int c = lane & 15;  // 16 bytes of a row
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k = 2 * i + (lane >> 4), src = 16 * kv + k;
+          const unsigned long long at = __shfl_sync(0xffffffffu, from, src) + 16 * c;
+          const uint32_t to = dst + (2 * kv + (c >> 3)) * kHalf + sw128(mrow + k, c & 7);
+          if (valid == 0xffffffffu)
+            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(to), "l"(at)
+                         : "memory");
+          else
+            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(to),
+                         "l"(at), "r"((valid >> src & 1) ? 16 : 0)
+                         : "memory");
+        }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      ++issued;
+      lkey += kRound;
+      if (lkey < lk1) {
+        lidx += step_pages;
+        lrow += step_rows;
+        if (a.paged && lrow >= a.page_size) {
+          lrow -= a.page_size;
+          ++lidx;
+        }
+        find_page();
+      } else {
+        opened = false;
+        ++ln;
+      }
+    };
+    while (issued < kRing - 1 && open(0)) issue();
     for (uint32_t n = 0;; ++n) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&work_full[n % kWorks], n / kWorks & 1));
+      if (!__all_sync(0xffffffffu, mbar_wait(&work_full[n % kWorks], n / kWorks & 1))) ok = false;
       if (group_or(1, kWarps * 32, !ok)) {  // all warps leave together
         ok = false;
         break;
       }
       const Work& w = works[n % kWorks];
       if (!w.live) break;
-      // rows r0, r1: keys that they see, queries as the A operand
+      // rows r0, r1 of the warp's fragments: keys that they see
       const int r0 = mrow + qr, r1 = r0 + 8;
       const int tok0 = r0 / grp, tok1 = r1 / grp;
       const bool in0 = r0 < g.sub * grp && tok0 < w.toks, in1 = r1 < g.sub * grp && tok1 < w.toks;
       const int lim0 = in0 ? max(w.lim0 + tok0, 0) : 0, lim1 = in1 ? max(w.lim0 + tok1, 0) : 0;
-      const __nv_bfloat16* q0 = a.q + (w.row0 + tok0) * a.q_stride +
-                                ((long long)w.head * grp + r0 % grp) * kHeadDim + 2 * qc;
-      const __nv_bfloat16* q1 = a.q + (w.row0 + tok1) * a.q_stride +
-                                ((long long)w.head * grp + r1 % grp) * kHeadDim + 2 * qc;
-      uint32_t qf[8][4];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        qf[i][0] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(q0 + 16 * i)) : 0u;
-        qf[i][1] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(q1 + 16 * i)) : 0u;
-        qf[i][2] = in0 ? __ldg(reinterpret_cast<const uint32_t*>(q0 + 16 * i + 8)) : 0u;
-        qf[i][3] = in1 ? __ldg(reinterpret_cast<const uint32_t*>(q1 + 16 * i + 8)) : 0u;
+      // the item's queries, as K and V: 64 columns of all rows, 128-byte swizzle
+      for (int i = tid; i < kRowsItem * 16; i += kWarps * 32) {
+        const int r = i >> 4, c = i & 15, tok = r / grp;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (r < g.sub * grp && tok < w.toks)
+          x = __ldg(reinterpret_cast<const uint4*>(a.q + (w.row0 + tok) * a.q_stride +
+                                                   ((long long)w.head * grp + r % grp) * kHeadDim) +
+                    c);
+        st_shared_v4(sq + (c >> 3) * kRowsItem * 128 + sw128(r, c & 7), x.x, x.y, x.z, x.w);
       }
+      group_sync(1, kWarps * 32);
       float o[16][4];
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
       const int first = w.k0 + group * kChunk;
       const uint32_t begun = done;
-      for (int key0 = first; key0 < w.k1; key0 += kTile) {
-        if (done > begun) {  // the stage before is free (the last one is kept for the join)
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&empty[group][(done - 1) % kRing]);
-        }
-        const uint32_t st = done % kRing;
-        ok = __all_sync(0xffffffffu, mbar_wait(&full[group][st], done / kRing & 1));
-        if (!ok) break;
+      for (int key0 = first; key0 < w.k1; key0 += kRound) {
+        while (issued < done + kRing - 1 && open(n)) issue();
+        static_assert(kRing == 2, "one chunk is on its way");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");  // this chunk has arrived
+        if constexpr (MT > 1) group_sync(2 + group, MT * 32);
+        else __syncwarp();
+        if (open(n)) issue();  // into the stage of the chunk before, which everyone has left
+        const uint32_t kb = stages + done % kRing * kStage, vb = kb + 2 * kHalf;
         ++done;
-        const uint32_t kb = ring0 + (group * kRing + st) * kStage, vb = kb + 2 * kHalf;
         float s[2 * MT][4];
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+          uint32_t qf[4];
+          ldmatrix4(sq + (i >> 2) * kRowsItem * 128 +
+                        sw128(mrow + (lane & 15), 2 * (i & 3) + (lane >> 4)), qf);
 #pragma unroll
           for (int c = 0; c < MT; ++c) {  // 16 keys
             uint32_t kf[4];
             const uint32_t key = 16 * c + (lane >> 4) * 8 + (lane & 7);
             ldmatrix4(kb + (i >> 2) * kHalf + sw128(key, 2 * (i & 3) + ((lane >> 3) & 1)), kf);
-            mma16816(s[2 * c], qf[i], kf[0], kf[1]);
-            mma16816(s[2 * c + 1], qf[i], kf[2], kf[3]);
+            mma16816(s[2 * c], qf, kf[0], kf[1]);
+            mma16816(s[2 * c + 1], qf, kf[2], kf[3]);
           }
         }
         const int c0 = key0 + 2 * qc;  // key of s[0][0]
@@ -315,26 +343,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           l0 += s[i][0] + s[i][1];
           l1 += s[i][2] + s[i][3];
         }
-        const bool tail = key0 + kChunk > w.kv_len;  // rows of V behind the last key: zeroed
 #pragma unroll
         for (int c = 0; c < MT; ++c) {
           const uint32_t pf[4] = {pack_bf16(s[2 * c][0], s[2 * c][1]),
                                   pack_bf16(s[2 * c][2], s[2 * c][3]),
                                   pack_bf16(s[2 * c + 1][0], s[2 * c + 1][1]),
                                   pack_bf16(s[2 * c + 1][2], s[2 * c + 1][3])};
-          uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-          if (tail) {
-            const int k = c0 + 16 * c;
-            keep0 = (k < w.kv_len ? 0xffffu : 0u) | (k + 1 < w.kv_len ? 0xffff0000u : 0u);
-            keep1 = (k + 8 < w.kv_len ? 0xffffu : 0u) | (k + 9 < w.kv_len ? 0xffff0000u : 0u);
-          }
 #pragma unroll
           for (int d = 0; d < 8; ++d) {  // 16 columns of V
             uint32_t vf[4];
             const uint32_t key = 16 * c + ((lane >> 3) & 1) * 8 + (lane & 7);
             ldmatrix4_trans(vb + (d >> 2) * kHalf + sw128(key, 2 * (d & 3) + (lane >> 4)), vf);
-            mma16816(o[2 * d], pf, vf[0] & keep0, vf[1] & keep1);
-            mma16816(o[2 * d + 1], pf, vf[2] & keep0, vf[3] & keep1);
+            mma16816(o[2 * d], pf, vf[0], vf[1]);
+            mma16816(o[2 * d + 1], pf, vf[2], vf[3]);
           }
         }
       }
@@ -353,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if constexpr (MT > 1) group_sync(2 + group, MT * 32);  // the others have read V
       if (has) {
-        const uint32_t base = ring0 + (group * kRing + last) * kStage;
+        const uint32_t base = stages + last * kStage;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const uint32_t c = 4 * (i ^ (qr & 3)) + qc;
@@ -371,8 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // join: 16 threads per row, 8 columns each
 #pragma unroll 1
-      for (int it = 0; it < MT; ++it) {
-        const int r = it * 16 + tid / 16, nt = tid % 16;
+      for (int r = tid / 16; r < kRowsItem; r += kWarps * 2) {
+        const int nt = tid % 16;
         float M = -INFINITY;
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) M = fmaxf(M, stat[k][r].x);
@@ -413,9 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             reinterpret_cast<float2*>(p.ws.stats(piece))[r] = make_float2(M, l);
         }
       }
-      fence_proxy_async();                 // the stages are next written by TMA
-      group_sync(1, kWarps * 32);          // everyone has read stages, statistics and the piece
-      if (lane == 0 && has) mbar_arrive(&empty[group][last]);
+      group_sync(1, kWarps * 32);  // everyone has read the stages, statistics and the piece
       if (w.slot >= 0) {
         const int head0 = w.head * grp;
         attn_join<kWarps, 2>(
@@ -430,6 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&work_empty[n % kWorks]);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok) {
       *failed = 1;
       if (lane == 0) atomicOr(&g_rows_error, kErrLoad);
@@ -449,20 +469,17 @@ cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long lo
   p.g.overhead = 128;
   p.g.whole = 4;
   p.ws = attn_partials(workspace, 16 * MT, tag);
-  p.box = attn_key_box(a, 16 * MT);
-  CUtensorMap mk, mv;
-  if (!attn_key_maps(&mk, &mv, a, p.box)) return cudaErrorInvalidValue;
   static thread_local int set_for = -1;  // the attribute belongs to the device's context
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (set_for != dev) {
     e = cudaFuncSetAttribute(attn_rows_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)kSmemBytes);
+                             (int)smem_bytes(16 * MT));
     if (e != cudaSuccess) return e;
     set_for = dev;
   }
-  attn_rows_kernel<MT><<<sms, kThreads, kSmemBytes, st>>>(mk, mv, p);
+  attn_rows_kernel<MT><<<sms, kThreads, smem_bytes(16 * MT), st>>>(p);
   return cudaGetLastError();
 }
 

@@ -253,7 +253,8 @@ __device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& l
   const int lane = threadIdx.x & 31;
   const long long end = start + e + g.overhead;
   int count = 0;
-  for (int c0 = 0; c0 < line.parts; c0 += 32) {
+  // (the CTA of cost `start` is not before this one: a range is at most per + 1 long)
+  for (int c0 = (int)(start / (line.per + 1)); c0 < line.parts && line.cut(c0) < end; c0 += 32) {
     const int c = c0 + lane;
     bool has = false;
     long long lo = 0;
