@@ -1,15 +1,20 @@
 // Causal softmax attention for few query rows: decode steps and draft tokens over a paged
 // cache (or very short prompts).  Bound by the HBM traffic of K and V.
 //
-// An item has up to R = 16, 32 or 64 rows: the query heads of one key/value head for as
-// many tokens as fit.  Every SM runs one CTA whose eight consumer warps split the keys:
-// with R = 16 MT, MT warps (16 rows each) share a chunk of 16 MT keys and there are 8 / MT
-// such groups.  Each group keeps a ring of three chunks in shared memory that its own lanes
-// fill by cp.async, two chunks ahead, across the ends of pieces (192 KB a CTA, 128 KB of them
-// in flight); a box of 16 keys is too small for TMA, whose issue then bounds the loads (2 KB
-// boxes measured 5.2 TB/s from eight lanes and 2.0 TB/s from one).  16 rows per mma.sync
-// m16n8k16: the tensor work is a few per cent of the time that the keys take to arrive, and a
-// 128-row tcgen05 tile would be mostly padding and a longer chain.
+// An item has up to R = 8, 16, 32 or 64 rows: the query heads of one key/value head for as
+// many tokens as fit.  Every SM runs one CTA whose twelve consumer warps split the keys: a
+// group of W warps shares a chunk of 16 W keys, each warp for 8 NT of the rows (R = 8 NT W).
+// Each group has two chunks in shared memory (192 KB a CTA) that its own lanes fill by
+// cp.async, the next one while they work, across the ends of pieces; a box of 16 keys is too
+// small for TMA, whose issue then bounds the loads (2 KB boxes measured 5.2 TB/s from eight
+// lanes and 2.0 TB/s from one).
+//
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, in mma.sync m16n8k16: the
+// keys (then the columns of V) fill the 16 and the rows the 8, so that a decode step's eight
+// heads of a group waste nothing, and a row's maximum, sum and scale stay in one thread's
+// columns.  P^T needs a transposed fragment, one movmatrix per 8 keys.  The warps are bound by
+// latency (the tensor pipe is 13 % busy): what counts is instructions per chunk and warps.
+// A 128-row tcgen05 tile would be mostly padding and a longer chain of hand-overs.
 //
 // Each warp keeps its own running maximum, sum and output in registers (raised lazily, as in
 // the tensor-core kernel); the groups are joined through shared memory at the end of a piece,
@@ -71,19 +76,25 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int MT>
+// An 8 x 8 matrix of bf16 (a row's column pair in each thread), transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <int W, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_rows_kernel(const __grid_constant__ RowsArgs p) {
-  constexpr int kGroups = kWarps / MT;
-  constexpr int kChunk = 16 * MT;              // keys
+  constexpr int kGroups = kWarps / W;
+  constexpr int kChunk = 16 * W;               // keys
   constexpr int kHalf = kChunk * 128;          // 64 columns of a chunk's K or V
-  constexpr int kStage = 4 * kHalf;            // K, V; also the size of a group's fp32 output
-  constexpr int kRowsItem = 16 * MT;
-  static_assert(kRowsItem * kHeadDim * 4 == kStage, "the join goes through a stage");
+  constexpr int kStage = 4 * kHalf;            // K, V
+  constexpr int kRowsItem = 8 * NT * W;
+  static_assert(kRowsItem * kHeadDim * 4 <= kStage, "the join goes through a stage");
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t work_full[kWorks], work_empty[kWorks];
+  __shared__ uint64_t work_full[kWorks], pieces_full[kWorks], work_empty[kWorks];
   __shared__ Work works[kWorks];
-  __shared__ AttnShare share;
   __shared__ float2 stat[kGroups][kRowsItem];  // (maximum, sum) of each group's rows
   __shared__ uint32_t kept[kGroups];           // the stage that holds a group's output
   __shared__ int failed_flag, joining;
@@ -98,15 +109,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < kWorks; ++i) {
       mbar_init(&work_full[i], 1);
+      mbar_init(&pieces_full[i], 1);
       mbar_init(&work_empty[i], kWarps);
     }
     fence_mbar_init();
     failed_flag = 0;
   }
-  attn_share<kThreads>(a, g, blockIdx.x, gridDim.x, &share);  // ends with __syncthreads
+  __syncthreads();
 
   if (warp == kWarps) {
     // ------------------------------------------------------------------ the pieces
+    const AttnShare share = attn_share(a, g, blockIdx.x, gridDim.x);
     const long long u0 = share.u0, u1 = share.u1;
     AttnCursor cur;
     bool more = u0 < u1;
@@ -117,7 +130,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       if (__any_sync(0xffffffffu, *failed)) break;
       Work* w = &works[n % kWorks];
-      bool found = false;
+      bool found = false, split = false;
+      long long start = 0;
+      int keys = 0;
       while (more && !found) {
         const int e = cur.keys(g), tiles = (e + kTile - 1) / kTile;
         const int t0 = attn_tile_at(g, e, tiles, u0 > cur.start ? u0 - cur.start : 0);
@@ -126,7 +141,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         found = t1 > t0 || (tiles == 0 && cur.start >= u0);
         if (found) {
           const int slot = (t0 == 0 && t1 == tiles) ? -1 : (u0 > cur.start ? 0 : 1);
-          if (slot >= 0) attn_pieces(g, share.line, cur.start, e, tiles, blockIdx.x, &w->pieces);
+          split = slot >= 0;
+          start = cur.start;
+          keys = e;
           if (lane == 0) {
             const int first = cur.b * g.block;
             w->row0 = cur.seq.q0 + first;
@@ -147,12 +164,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&work_full[n % kWorks]);
       if (!found) break;
+      // needed at the piece's end only
+      if (split)
+        attn_pieces(g, share.line, start, keys, (keys + kTile - 1) / kTile, blockIdx.x, &w->pieces);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pieces_full[n % kWorks]);
     }
   } else {
     // ------------------------------------------------------------------ consumers
-    const int group = warp / MT;
-    const int mrow = (warp % MT) * 16;             // first row of the warp's tile
-    const int qr = lane >> 2, qc = lane & 3;       // rows qr, qr + 8; column pair of a fragment
+    const int group = warp / W;
+    const int mkey = (warp % W) * 16;              // the chunk's keys that the warp loads
+    const int mrow = (warp % W) * 8 * NT;          // its first row
+    const int fr = lane >> 2, fc = 2 * (lane & 3);  // row and column pair of a fragment
     const uint32_t stages = ring0 + group * kRing * kStage;
     uint32_t done = 0;  // chunks consumed
     bool ok = true;
@@ -172,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int step_pages = a.paged ? kRound / a.page_size : 0;
     const int step_rows = kRound - step_pages * (a.paged ? a.page_size : 0);
     auto find_page = [&] {  // asked for a chunk ahead of its use
-      if (a.paged) page = lkey + mrow + (lane & 15) < lend ? __ldg(ltable + lidx) : -1;
+      if (a.paged) page = lkey + mkey + (lane & 15) < lend ? __ldg(ltable + lidx) : -1;
     };
     // To the next chunk; `n` is the piece at hand (a wait for one kWorks later would not end).
     auto open = [&](uint32_t n) {
@@ -189,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           opened = true;
           lend = w.kv_len;
           lkv0 = w.kv0;
-          const int key = lkey + mrow + (lane & 15);
+          const int key = lkey + mkey + (lane & 15);
           lidx = a.paged ? key / a.page_size : 0;
           lrow = a.paged ? key - lidx * a.page_size : lkv0 + key;
           lbase = (lane < 16 ? a.k : a.v) + (long long)w.head * kHeadDim;
@@ -202,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       return opened;
     };
     auto issue = [&] {  // its loads: keys behind the last one and missing pages become zeros
-      const bool there = lkey + mrow + (lane & 15) < lend &&
+      const bool there = lkey + mkey + (lane & 15) < lend &&
                          (!a.paged || (page >= 0 && page < a.num_pages));
       const unsigned long long from = reinterpret_cast<unsigned long long>(
           there ? lbase + page * page_stride + lrow * row_stride : a.k);
@@ -215,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 8; ++i) {
           const int k = 2 * i + (lane >> 4), src = 16 * kv + k;
           const unsigned long long at = __shfl_sync(0xffffffffu, from, src) + 16 * c;
-          const uint32_t to = dst + (2 * kv + (c >> 3)) * kHalf + sw128(mrow + k, c & 7);
+          const uint32_t to = dst + (2 * kv + (c >> 3)) * kHalf + sw128(mkey + k, c & 7);
           if (valid == 0xffffffffu)
             asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(to), "l"(at)
                          : "memory");
@@ -249,11 +272,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const Work& w = works[n % kWorks];
       if (!w.live) break;
-      // rows r0, r1 of the warp's fragments: keys that they see
-      const int r0 = mrow + qr, r1 = r0 + 8;
-      const int tok0 = r0 / grp, tok1 = r1 / grp;
-      const bool in0 = r0 < g.sub * grp && tok0 < w.toks, in1 = r1 < g.sub * grp && tok1 < w.toks;
-      const int lim0 = in0 ? max(w.lim0 + tok0, 0) : 0, lim1 = in1 ? max(w.lim0 + tok1, 0) : 0;
       // the item's queries, as K and V: 64 columns of all rows, 128-byte swizzle
       for (int i = tid; i < kRowsItem * 16; i += kWarps * 32) {
         const int r = i >> 4, c = i & 15, tok = r / grp;
@@ -265,126 +283,150 @@ __global__ void __launch_bounds__(kThreads, 1)
         st_shared_v4(sq + (c >> 3) * kRowsItem * 128 + sw128(r, c & 7), x.x, x.y, x.z, x.w);
       }
       group_sync(1, kWarps * 32);
-      float o[16][4];
+      // the thread's rows (columns of the transposed products) are mrow + 8 t + fc and the
+      // next one: keys that they see.  One tile of rows keeps its queries, the B operand, in
+      // registers; two would spill (216 bytes).
+      int lim[NT][2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int r = mrow + 8 * t + fc + k, tok = r / grp;
+          lim[t][k] = r < g.sub * grp && tok < w.toks ? max(w.lim0 + tok, 0) : 0;
+        }
+      const int qrow = NT == 1 ? mrow + (lane & 7) : mrow + 8 * (lane >> 4) + (lane & 7);
+      uint32_t qk[NT == 1 ? 4 : 1][4];
+      if constexpr (NT == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // two steps of 16 columns
+          ldmatrix4(sq + (i >> 1) * kRowsItem * 128 + sw128(qrow, 4 * (i & 1) + (lane >> 3)), qk[i]);
+      }
+      float o[NT][8][4], m[NT][2], l[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        m[t][0] = m[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+      }
       const int first = w.k0 + group * kChunk;
       const uint32_t begun = done;
       for (int key0 = first; key0 < w.k1; key0 += kRound) {
         while (issued < done + kRing - 1 && open(n)) issue();
         static_assert(kRing == 2, "one chunk is on its way");
         asm volatile("cp.async.wait_group 0;" ::: "memory");  // this chunk has arrived
-        if constexpr (MT > 1) group_sync(2 + group, MT * 32);
+        if constexpr (W > 1) group_sync(2 + group, W * 32);
         else __syncwarp();
         if (open(n)) issue();  // into the stage of the chunk before, which everyone has left
         const uint32_t kb = stages + done % kRing * kStage, vb = kb + 2 * kHalf;
         ++done;
-        float s[2 * MT][4];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int c = 0; c < W; ++c) {  // 16 keys
+          float s[NT][4], s2[NT][4];   // two chains of four products
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t qf[4];
-          ldmatrix4(sq + (i >> 2) * kRowsItem * 128 +
-                        sw128(mrow + (lane & 15), 2 * (i & 3) + (lane >> 4)), qf);
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int c = 0; c < MT; ++c) {  // 16 keys
+            for (int k = 0; k < 4; ++k) s[t][k] = s2[t][k] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
             uint32_t kf[4];
-            const uint32_t key = 16 * c + (lane >> 4) * 8 + (lane & 7);
-            ldmatrix4(kb + (i >> 2) * kHalf + sw128(key, 2 * (i & 3) + ((lane >> 3) & 1)), kf);
-            mma16816(s[2 * c], qf, kf[0], kf[1]);
-            mma16816(s[2 * c + 1], qf, kf[2], kf[3]);
+            ldmatrix4(kb + (i >> 2) * kHalf + sw128(16 * c + (lane & 15), 2 * (i & 3) + (lane >> 4)),
+                      kf);
+            if constexpr (NT == 1) {
+              mma16816((i & 1) ? s2[0] : s[0], kf, qk[i >> 1][2 * (i & 1)],
+                       qk[i >> 1][2 * (i & 1) + 1]);
+            } else {
+              uint32_t qf[4];
+              ldmatrix4(sq + (i >> 2) * kRowsItem * 128 +
+                            sw128(qrow, 2 * (i & 3) + ((lane >> 3) & 1)),
+                        qf);
+              mma16816((i & 1) ? s2[0] : s[0], kf, qf[0], qf[1]);
+              mma16816((i & 1) ? s2[1] : s[1], kf, qf[2], qf[3]);
+            }
           }
-        }
-        const int c0 = key0 + 2 * qc;  // key of s[0][0]
-        if (__any_sync(0xffffffffu, key0 + kChunk > lim0 || key0 + kChunk > lim1)) {
+          const int k0 = key0 + 16 * c + fr;  // key of s[.][0], s[.][1]; k0 + 8 of the others
+          bool up = false;
 #pragma unroll
-          for (int i = 0; i < 2 * MT; ++i) {
-            s[i][0] = c0 + 8 * i < lim0 ? s[i][0] : -INFINITY;
-            s[i][1] = c0 + 8 * i + 1 < lim0 ? s[i][1] : -INFINITY;
-            s[i][2] = c0 + 8 * i < lim1 ? s[i][2] : -INFINITY;
-            s[i][3] = c0 + 8 * i + 1 < lim1 ? s[i][3] : -INFINITY;
+          for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              s[t][k] = (s[t][k] + s2[t][k]) * a.scale_log2;
+              if (k0 + (k & 2) * 4 >= lim[t][k & 1]) s[t][k] = -INFINITY;
+            }
+            up = up || fmaxf(s[t][0], s[t][2]) > m[t][0] + kRaise ||
+                 fmaxf(s[t][1], s[t][3]) > m[t][1] + kRaise;
           }
-        }
-        float x0 = fmaxf(s[0][0], s[0][1]), x1 = fmaxf(s[0][2], s[0][3]);
+          if (__any_sync(0xffffffffu, up)) {  // some row's maximum has to be raised
 #pragma unroll
-        for (int i = 1; i < 2 * MT; ++i) {
-          x0 = fmaxf(x0, fmaxf(s[i][0], s[i][1]));
-          x1 = fmaxf(x1, fmaxf(s[i][2], s[i][3]));
-        }
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2)) * a.scale_log2;
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2)) * a.scale_log2;
-        const bool up0 = x0 > m0 + kRaise, up1 = x1 > m1 + kRaise;
-        if (__any_sync(0xffffffffu, up0 || up1)) {
-          const float f0 = up0 ? (m0 == -INFINITY ? 0.f : ex2(m0 - x0)) : 1.f;
-          const float f1 = up1 ? (m1 == -INFINITY ? 0.f : ex2(m1 - x1)) : 1.f;
-          if (up0) m0 = x0;
-          if (up1) m1 = x1;
-          l0 *= f0;
-          l1 *= f1;
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            o[i][0] *= f0;
-            o[i][1] *= f0;
-            o[i][2] *= f1;
-            o[i][3] *= f1;
+              for (int k = 0; k < 2; ++k) {
+                float x = fmaxf(s[t][k], s[t][k + 2]);
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                x = fmaxf(x, m[t][k]);
+                const float f = m[t][k] == -INFINITY ? 0.f : ex2(m[t][k] - x);
+                m[t][k] = x;
+                l[t][k] *= f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[t][i][k] *= f;
+                  o[t][i][k + 2] *= f;
+                }
+              }
           }
-        }
-        const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+          uint32_t pf[NT][2];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-          s[i][0] = ex2(fmaf(s[i][0], a.scale_log2, -b0));
-          s[i][1] = ex2(fmaf(s[i][1], a.scale_log2, -b0));
-          s[i][2] = ex2(fmaf(s[i][2], a.scale_log2, -b1));
-          s[i][3] = ex2(fmaf(s[i][3], a.scale_log2, -b1));
-          l0 += s[i][0] + s[i][1];
-          l1 += s[i][2] + s[i][3];
-        }
+          for (int t = 0; t < NT; ++t) {
 #pragma unroll
-        for (int c = 0; c < MT; ++c) {
-          const uint32_t pf[4] = {pack_bf16(s[2 * c][0], s[2 * c][1]),
-                                  pack_bf16(s[2 * c][2], s[2 * c][3]),
-                                  pack_bf16(s[2 * c + 1][0], s[2 * c + 1][1]),
-                                  pack_bf16(s[2 * c + 1][2], s[2 * c + 1][3])};
+            for (int k = 0; k < 4; ++k) {
+              s[t][k] = ex2(s[t][k] - (m[t][k & 1] == -INFINITY ? 0.f : m[t][k & 1]));
+              l[t][k & 1] += s[t][k];
+            }
+            pf[t][0] = transpose8x8(pack_bf16(s[t][0], s[t][1]));
+            pf[t][1] = transpose8x8(pack_bf16(s[t][2], s[t][3]));
+          }
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {  // 16 columns of V
+          for (int i = 0; i < 8; ++i) {  // 16 columns of V
             uint32_t vf[4];
-            const uint32_t key = 16 * c + ((lane >> 3) & 1) * 8 + (lane & 7);
-            ldmatrix4_trans(vb + (d >> 2) * kHalf + sw128(key, 2 * (d & 3) + (lane >> 4)), vf);
-            mma16816(o[2 * d], pf, vf[0], vf[1]);
-            mma16816(o[2 * d + 1], pf, vf[2], vf[3]);
+            ldmatrix4_trans(vb + (i >> 2) * kHalf + sw128(16 * c + (lane >> 4) * 8 + (lane & 7),
+                                                          2 * (i & 3) + ((lane >> 3) & 1)),
+                            vf);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma16816(o[t][i], vf, pf[t][0], pf[t][1]);
           }
         }
       }
-      // the group's result into the stage that it consumed last: row r's column pair c at
-      // pair c ^ 4 (r % 4) (two rows of lanes to a bank otherwise)
+      // the group's result into the stage that it consumed last: column d of row r at
+      // d ^ 8 (r / 2 % 4), so that a store's rows fall on different banks
       const bool has = done > begun;
       const uint32_t last = (done - 1) % kRing;
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
       if (lane == 0) kept[group] = last;  // the same from each of the group's warps
-      if (qc == 0) {
-        stat[group][r0] = make_float2(has ? m0 : -INFINITY, l0);
-        stat[group][r1] = make_float2(has ? m1 : -INFINITY, l1);
-      }
-      if constexpr (MT > 1) group_sync(2 + group, MT * 32);  // the others have read V
-      if (has) {
-        const uint32_t base = stages + last * kStage;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t c = 4 * (i ^ (qr & 3)) + qc;
-          asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(base + r0 * 512 + 8 * c),
-                       "f"(o[i][0]), "f"(o[i][1])
-                       : "memory");
-          asm volatile("st.shared.v2.f32 [%0], {%1,%2};" ::"r"(base + r1 * 512 + 8 * c),
-                       "f"(o[i][2]), "f"(o[i][3])
-                       : "memory");
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float x = l[t][k];
+          x += __shfl_xor_sync(0xffffffffu, x, 4);
+          x += __shfl_xor_sync(0xffffffffu, x, 8);
+          x += __shfl_xor_sync(0xffffffffu, x, 16);
+          if (fr == 0) stat[group][mrow + 8 * t + fc + k] = make_float2(m[t][k], x);
         }
+      if constexpr (W > 1) group_sync(2 + group, W * 32);  // the others have read V
+      if (has) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int r = mrow + 8 * t + fc + (k & 1), d = 16 * i + fr + (k & 2) * 4;
+              asm volatile("st.shared.f32 [%0], %1;" ::"r"(stages + last * kStage + r * 512 +
+                                                           4 * (d ^ ((r >> 1 & 3) << 3))),
+                           "f"(o[t][i][k])
+                           : "memory");
+            }
       }
       if (group_or(1, kWarps * 32, !ok)) {
         ok = false;
@@ -404,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (ml.y == 0.f) continue;  // saw nothing
           const float f = ex2(ml.x - M);
           const uint32_t src = ring0 + (k * kRing + kept[k]) * kStage + r * 512 +
-                               32 * (nt ^ (r & 3));
+                               32 * (nt ^ (r >> 1 & 3));
           const uint4 u = ld_shared_v4(src), v = ld_shared_v4(src + 16);
           l = fmaf(f, ml.y, l);
           x[0] = fmaf(f, __uint_as_float(u.x), x[0]);
@@ -434,7 +476,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             reinterpret_cast<float2*>(p.ws.stats(piece))[r] = make_float2(M, l);
         }
       }
-      group_sync(1, kWarps * 32);  // everyone has read the stages, statistics and the piece
+      // (every thread waits for every piece: the phases stay in step)
+      if (!__all_sync(0xffffffffu, mbar_wait(&pieces_full[n % kWorks], n / kWorks & 1))) ok = false;
+      if (group_or(1, kWarps * 32, !ok)) {  // everyone has read the stages and statistics
+        ok = false;
+        break;
+      }
       if (w.slot >= 0) {
         const int head0 = w.head * grp;
         attn_join<kWarps, 2>(
@@ -457,29 +504,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int MT>
+template <int W, int NT>
 cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long long tag,
                    cudaStream_t st) {
   const int grp = a.hq / a.hkv;
   RowsArgs p{};
   p.a = a;
-  p.g.sub = 16 * MT / grp;
+  constexpr int rows = 8 * NT * W;
+  p.g.sub = rows / grp;
   p.g.block = p.g.sub;
-  p.g.sub_rows = 16 * MT;
   p.g.overhead = 128;
-  p.g.whole = 4;
-  p.ws = attn_partials(workspace, 16 * MT, tag);
+  p.g.whole = 8;
+  p.ws = attn_partials(workspace, rows, tag);
   static thread_local int set_for = -1;  // the attribute belongs to the device's context
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (set_for != dev) {
-    e = cudaFuncSetAttribute(attn_rows_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem_bytes(16 * MT));
+    e = cudaFuncSetAttribute(attn_rows_kernel<W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem_bytes(rows));
     if (e != cudaSuccess) return e;
     set_for = dev;
   }
-  attn_rows_kernel<MT><<<sms, kThreads, smem_bytes(16 * MT), st>>>(p);
+  attn_rows_kernel<W, NT><<<sms, kThreads, smem_bytes(rows), st>>>(p);
   return cudaGetLastError();
 }
 
@@ -497,9 +544,10 @@ unsigned read_attn_rows_error(bool clear) {
 
 cudaError_t launch_attn_rows(const AttnArgs& p, int rows, int sms, void* workspace,
                              unsigned long long tag, cudaStream_t st) {
-  return rows == 16   ? launch<1>(p, sms, workspace, tag, st)
-         : rows == 32 ? launch<2>(p, sms, workspace, tag, st)
-                      : launch<4>(p, sms, workspace, tag, st);
+  return rows == 8    ? launch<1, 1>(p, sms, workspace, tag, st)
+         : rows == 16 ? launch<1, 2>(p, sms, workspace, tag, st)
+         : rows == 32 ? launch<2, 2>(p, sms, workspace, tag, st)
+                      : launch<4, 2>(p, sms, workspace, tag, st);
 }
 
 }  // namespace gdn

@@ -23,11 +23,16 @@ constexpr int kAttnMaxParts = 160;  // CTAs that share the work (one per SM)
 
 struct AttnGrid {
   int block;     // query tokens per item
-  int sub;       // query tokens per tile of rows: row (tok / sub) * sub_rows + (tok % sub) *
-  int sub_rows;  // heads of the group + head
+  int sub;       // query tokens per tile of rows
   int overhead;  // cost of an item's start and end, in keys
   int whole;     // items of at most this many tiles are not split
 };
+
+// Quotients of costs: 32 bits where they do (a 64-bit division is some 100 instructions).
+__device__ __forceinline__ long long attn_div(long long x, long long y) {
+  if (((x | y) >> 32) == 0) return (unsigned)x / (unsigned)y;
+  return x / y;
+}
 
 // Keys that block b of a sequence reads.
 __device__ __forceinline__ int attn_block_keys(const AttnSeq& s, int block, int b) {
@@ -44,7 +49,7 @@ __device__ __forceinline__ long long attn_cost_before(const AttnSeq& s, const At
   const int nb = attn_blocks(s, g.block);
   const long long a = (long long)s.kv_len - s.q_len;
   const long long m = n < nb ? n : nb - 1;              // blocks of full size
-  long long b0 = a < 0 ? -a / g.block : 0;              // leading blocks that see nothing
+  long long b0 = a < 0 ? (unsigned)-a / (unsigned)g.block : 0;              // leading blocks that see nothing
   if (b0 > m) b0 = m;
   long long c = (m - b0) * a + (long long)g.block * ((m * (m + 1) - b0 * (b0 + 1)) / 2);
   if (n == nb) c += s.kv_len;
@@ -79,7 +84,7 @@ struct AttnCursor {
                                        long long at, long long u) {
     open(p, g, seq_index);
     const long long per = attn_head_cost(seq, g);
-    h = (int)((u - at) / per);
+    h = (int)attn_div(u - at, per);
     const long long r = u - at - h * per;
     int lo = 0, hi = nb - 1;  // the last block whose cost begins at or before r
     while (lo < hi) {
@@ -125,77 +130,49 @@ struct AttnShare {
   int seq;
 };
 
-// Collective over a block of NT threads (a multiple of 32): the share of CTA c of `parts`.
-template <int NT>
-__device__ __forceinline__ void attn_share(const AttnArgs& p, const AttnGrid& g, int c, int parts,
-                                           AttnShare* out) {
-  __shared__ long long warp_sum[NT / 32];
-  __shared__ int found;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool one = p.num_seqs <= NT;  // a sequence a thread: one pass finds everything
-  long long mine = 0;
-  for (int s = tid; s < p.num_seqs; s += NT) mine += attn_head_cost(attn_seq(p, s), g) * p.hkv;
-  long long sum = mine;  // inclusive over the threads
+// By one warp: the share of CTA c of `parts`.
+__device__ __forceinline__ AttnShare attn_share(const AttnArgs& p, const AttnGrid& g, int c,
+                                                int parts) {
+  const int lane = threadIdx.x & 31;
+  AttnShare r;
+  long long cost = 0, mine = 0;  // of the lane's last sequence, of all of them
+#pragma unroll 4
+  for (int s = lane; s < p.num_seqs; s += 32) {
+    cost = attn_head_cost(attn_seq(p, s), g) * p.hkv;
+    mine += cost;
+  }
 #pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, sum, w);
-    if (lane >= w) sum += y;
-  }
-  if (lane == 31) warp_sum[warp] = sum;
-  __syncthreads();
-  AttnLine line;
-  line.total = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 32; ++w) {
-    if (w == warp) sum += line.total;
-    line.total += warp_sum[w];
-  }
-  line.per = line.total / parts;
-  line.rest = (int)(line.total - line.per * parts);
-  line.parts = parts;
-  const long long u = line.cut(c);
-  if (tid == 0) {
-    out->line = line;
-    out->u0 = u;
-    out->u1 = line.cut(c + 1);
-    found = 0;
-  }
-  if (one) {
-    if (sum - mine <= u && u < sum) {
-      out->seq = tid;
-      out->seq_start = sum - mine;
+  for (int w = 1; w < 32; w <<= 1) mine += __shfl_xor_sync(0xffffffffu, mine, w);
+  r.line.total = mine;
+  r.line.per = attn_div(mine, parts);
+  r.line.rest = (int)(mine - r.line.per * parts);
+  r.line.parts = parts;
+  r.u0 = r.line.cut(c);
+  r.u1 = r.line.cut(c + 1);
+  r.seq = 0;
+  r.seq_start = 0;
+  if (r.u0 >= r.u1) return r;  // no work: the line is shorter than the number of CTAs
+  long long base = 0;
+  for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
+    if (p.num_seqs > 32) {
+      cost = s0 + lane < p.num_seqs ? attn_head_cost(attn_seq(p, s0 + lane), g) * p.hkv : 0;
     }
-  } else {
-    long long base = 0;
-    for (int s0 = 0; s0 < p.num_seqs && u < line.total; s0 += NT) {
-      __syncthreads();
-      if (found) break;
-      const int s = s0 + tid;
-      const long long x = s < p.num_seqs ? attn_head_cost(attn_seq(p, s), g) * p.hkv : 0;
-      sum = x;
+    long long sum = base + cost;
 #pragma unroll
-      for (int w = 1; w < 32; w <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, sum, w);
-        if (lane >= w) sum += y;
-      }
-      if (lane == 31) warp_sum[warp] = sum;
-      __syncthreads();
-      long long all = 0;
-#pragma unroll
-      for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) sum += warp_sum[w];
-        all += warp_sum[w];
-      }
-      sum += base;
-      if (x > 0 && sum - x <= u && u < sum) {
-        out->seq = s;
-        out->seq_start = sum - x;
-        found = 1;
-      }
-      base += all;
+    for (int w = 1; w < 32; w <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, sum - base, w);
+      if (lane >= w) sum += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, sum > r.u0);
+    base = __shfl_sync(0xffffffffu, sum, 31);
+    if (past != 0) {  // the first sequence that ends behind u0
+      const int at = __ffs(past) - 1;
+      r.seq = s0 + at;
+      r.seq_start = __shfl_sync(0xffffffffu, sum - cost, at);
+      break;
     }
   }
-  __syncthreads();
+  return r;
 }
 
 // ---------------------------------------------------------------- partial results
@@ -254,7 +231,7 @@ __device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& l
   const long long end = start + e + g.overhead;
   int count = 0;
   // (the CTA of cost `start` is not before this one: a range is at most per + 1 long)
-  for (int c0 = (int)(start / (line.per + 1)); c0 < line.parts && line.cut(c0) < end; c0 += 32) {
+  for (int c0 = (int)attn_div(start, line.per + 1); c0 < line.parts && line.cut(c0) < end; c0 += 32) {
     const int c = c0 + lane;
     bool has = false;
     long long lo = 0;
@@ -309,7 +286,7 @@ __device__ __forceinline__ void attn_merge(const AttnPartials& ws, const short* 
     for (int j = 0; j < R; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
-#pragma unroll 2
+#pragma unroll(R > 2 ? 2 : 8)  // loads of 16 rows in flight
       for (int i = 0; i < kPer; ++i) {
         if (k * kPer + i >= count) break;
         const float* src = ws.sums(list[(k * kPer + i) * step]) +
@@ -350,9 +327,9 @@ __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPiec
                                           Sync&& sync, Store&& store) {
   const int lane = threadIdx.x & 31;
   auto arrive = [&](int first, int level, int n) {  // true in the last CTA to arrive
-    __threadfence();
-    sync();
+    sync();  // the others' rows before this thread's fence
     if (warp == 0 && lane == 0) {
+      __threadfence();
       *flag = attn_arrive(&ws.counters->arrived[pieces.list[first]][level][tile], ws.tag, n);
       __threadfence();
     }

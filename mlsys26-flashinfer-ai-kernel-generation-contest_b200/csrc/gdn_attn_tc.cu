@@ -61,7 +61,6 @@ struct Work {
 };
 struct Shared {
   Bars bars;
-  AttnShare share;
   Work work[kWorks];
   uint32_t tmem;
   int failed, joining[2];
@@ -162,7 +161,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
-  attn_share<kThreads>(a, g, blockIdx.x, gridDim.x, &sh.share);  // ends with __syncthreads
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -176,9 +174,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 10) {
       // ------------------------------------------------------------------ the pieces
+      const AttnShare share = attn_share(a, g, blockIdx.x, gridDim.x);
       AttnCursor cur;
-      bool more = sh.share.u0 < sh.share.u1;
-      if (more) cur.seek(a, g, sh.share.seq, sh.share.seq_start, sh.share.u0);
+      bool more = share.u0 < share.u1;
+      if (more) cur.seek(a, g, share.seq, share.seq_start, share.u0);
       for (uint32_t n = 0;; ++n) {
         if (n >= kWorks && !__all_sync(0xffffffffu, mbar_wait(&bars.work_empty[n % kWorks],
                                                               (n / kWorks - 1) & 1)))
@@ -187,8 +186,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         Work* w = &sh.work[n % kWorks];
         bool found = false;
         while (more && !found) {
-          found = piece_of(cur, g, sh.share, w);
-          more = cur.next(a, g) && cur.start < sh.share.u1;
+          found = piece_of(cur, g, share, w);
+          more = cur.next(a, g) && cur.start < share.u1;
         }
         if (lane == 0 && !found) w->live = false;
         __syncwarp();
@@ -565,7 +564,6 @@ cudaError_t launch_attn_tc(const AttnArgs& a, int sms, void* workspace, unsigned
   p.a = a;
   p.g.sub = kRows / grp;
   p.g.block = 2 * p.g.sub;
-  p.g.sub_rows = kRows;
   p.g.overhead = 128;
   p.g.whole = 4;
   p.ws = attn_partials(workspace, 2 * kRows, tag);
