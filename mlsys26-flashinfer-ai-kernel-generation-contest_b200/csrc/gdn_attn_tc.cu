@@ -44,6 +44,7 @@ struct Bars {
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t s_full[2], p_ready[2], o_full[2];
   uint64_t work_full[kWorks], work_empty[kWorks];
+  uint64_t twin_ready, twin_done;
   uint64_t drain;
 };
 // One piece of an item, for all roles.
@@ -56,6 +57,7 @@ struct Work {
   int t0, t1;      // key tiles of the piece
   int end[2];      // of which row tile 0 / 1 needs those below
   int slot;        // partial results' slot, -1: the piece is the whole item
+  bool twin;       // one row tile: both halves of the CTA work on it, on key tiles in turn
   bool live;       // false: behind the last one
   AttnPieces pieces;  // of the item, where it has more than this one
 };
@@ -64,6 +66,7 @@ struct Shared {
   Work work[kWorks];
   uint32_t tmem;
   int failed, joining[2];
+  float2 twin[kRows];  // (maximum, sum) of the second half's rows
 };
 constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + kStages * kTileBytes;
 
@@ -105,6 +108,7 @@ __device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& 
     w->end[t] = min(t1, sees > 0 ? (sees + kTile - 1) / kTile : 0);
   }
   w->slot = slot;
+  w->twin = w->toks <= g.sub;
   w->live = true;
   return true;
 }
@@ -150,6 +154,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&b.work_full[i], 1);
       mbar_init(&b.work_empty[i], 10);  // loader, issuer, eight softmax warps
     }
+    mbar_init(&b.twin_ready, 128);
+    mbar_init(&b.twin_done, 128);
     mbar_init(&b.drain, 1);
     fence_mbar_init();
     sh.failed = 0;
@@ -283,9 +289,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) why = err;
           if (*failed) ok = false;
         };
-        auto scores = [&](int t, uint32_t entry) {  // S_t = Q_t K^T
+        auto scores = [&](int t, int qt, uint32_t entry) {  // S_t = Q_qt K^T
           const uint32_t k = skv + entry % kStages * kTileBytes;
-          const uint32_t q = sq + t * kTileBytes;
+          const uint32_t q = sq + qt * kTileBytes;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint32_t off = (i >> 2) * kHalfBytes + (i & 3) * 32;
@@ -305,15 +311,45 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok || !sh.work[n % kWorks].live) break;
           const int t0 = sh.work[n % kWorks].t0, t1 = sh.work[n % kWorks].t1;
           const int end0 = sh.work[n % kWorks].end[0], end1 = sh.work[n % kWorks].end[1];
+          const bool twin = sh.work[n % kWorks].twin;
           mbar_arrive(&bars.work_empty[n % kWorks]);
           if (t1 <= t0) continue;
+          if (twin) {
+            // key tile j goes to half (j - t0) % 2; its scores are taken two tiles ahead
+            wait(&bars.q_full[0], nq0++, kErrLoad);
+            auto ahead = [&](int j) {
+              const uint32_t e = 2 * (tile0 + j - t0);
+              wait(&bars.kv_full[e % kStages], e / kStages, kErrLoad);
+              if (!ok) return;
+              tc_fence_after();
+              scores((j - t0) & 1, 0, e);
+              umma_commit(&bars.kv_empty[e % kStages]);
+              if (j + 1 == t1) umma_commit(&bars.q_empty);
+            };
+            ahead(t0);
+            if (t0 + 1 < t1) ahead(t0 + 1);
+            for (int j = t0; j < t1 && ok; ++j) {
+              const uint32_t e = 2 * (tile0 + j - t0) + 1;
+              const int t = (j - t0) & 1;
+              wait(&bars.kv_full[e % kStages], e / kStages, kErrLoad);
+              wait(&bars.p_ready[t], t ? np1++ : np0++, kErrTensor);
+              if (!ok) break;
+              tc_fence_after();
+              values(t, e, j < t0 + 2);
+              umma_commit(&bars.kv_empty[e % kStages]);
+              if (j + 2 < t1) ahead(j + 2);
+              else umma_commit(&bars.o_full[t]);
+            }
+            tile0 += t1 - t0;
+            continue;
+          }
           // the row tile that holds the block's last token needs every key tile: it comes last
           // and releases what both have read
           const int last = end1 == t1 ? 1 : 0;
           uint32_t entry = 2 * tile0;
           wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
           auto begin = [&](int t) {  // scores of tile j into S_t; K and, at the end, Q released
-            scores(t, entry);
+            scores(t, t, entry);
             if (t == last) umma_commit(&bars.kv_empty[entry % kStages]);
           };
           if (end0 > t0) {
@@ -371,22 +407,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = tid & 127;        // row
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane field: 32 (warp % 4)
     const uint32_t ts = tmem + 128 * t + lanes, to = tmem + 256 + 128 * t + lanes;
-    const int rtok = t * g.sub + r / grp;  // token of the block
-    uint32_t ns = 0, no = 0, tile0 = 0;
+    uint32_t ns = 0, no = 0, nt = 0, tile0 = 0;
     bool ok = true;
     for (uint32_t n = 0;; ++n) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1));
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1))) ok = false;
       if (group_or(1 + t, 128, !ok)) {  // the four warps leave together
         ok = false;
         break;
       }
       const Work& w = sh.work[n % kWorks];
       if (!w.live) break;
+      const bool twin = w.twin;
+      const int rt = twin ? 0 : t;            // row tile
+      const int rtok = rt * g.sub + r / grp;  // token of the block
       const bool mine = r < g.sub * grp && rtok < w.toks;
       const int lim = mine ? max(w.lim0 + rtok, 0) : 0;  // keys that the row sees
-      const int kv_len = w.kv_len, t0 = w.t0, t1 = w.end[t];
+      const int kv_len = w.kv_len, t0 = w.t0, t1 = w.end[rt];
+      const int jb = twin ? t0 + t : t0, step = twin ? 2 : 1;  // this half's key tiles
       float m = -INFINITY, l = 0.f;  // m in log2 units
-      for (int j = t0; j < t1; ++j) {
+      for (int j = jb; j < t1; j += step) {
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], ns++ & 1));
         if (!ok) break;
         tc_fence_after();
@@ -412,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float m2 = raise ? mx : m;
           const float f = m == -INFINITY ? 0.f : ex2(m - m2);
           l *= f;
-          if (j > t0) {  // O holds earlier tiles: their product is complete (s_full came after)
+          if (j > jb) {  // O holds earlier tiles: their product is complete (s_full came after)
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {  // 16 columns at a time: few registers, rare
               uint32_t o[16];
@@ -459,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bars.p_ready[t]);
         if (!ok) break;
       }
-      if (t1 > t0 && ok)
+      if (t1 > jb && ok)
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[t], no++ & 1));
       if (group_or(1 + t, 128, !ok)) {
         ok = false;
@@ -467,52 +506,83 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const int slot = w.slot;
-      const bool saw = mine && lim > t0 * kTile;  // some key of the piece
-      if (slot < 0) {
-        const float inv = 1.f / l;
-        __nv_bfloat16* op = a.out + (w.row0 + rtok) * a.o_stride +
-                            ((long long)w.head * grp + r % grp) * kHeadDim;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          if (t1 > t0) {
+      const bool has = t1 > jb;  // O_t holds something
+      if (twin && t == 1) {      // the first half reads this half's rows and finishes them
+        sh.twin[r] = has ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        tc_fence_before();
+        mbar_arrive(&bars.twin_ready);
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars.twin_done, nt++ & 1))) ok = false;
+      } else {
+        float f0 = 1.f, f1 = 0.f;  // weights of O_t and, for twins, of O_1
+        if (twin) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&bars.twin_ready, nt++ & 1))) ok = false;
+          tc_fence_after();
+          const float2 x = sh.twin[r];
+          const float top = fmaxf(l == 0.f ? -INFINITY : m, x.y == 0.f ? -INFINITY : x.x);
+          f0 = l == 0.f ? 0.f : ex2(m - top);
+          f1 = x.y == 0.f ? 0.f : ex2(x.x - top);
+          l = f0 * l + f1 * x.y;
+          m = top;
+        }
+        const bool both = twin && t1 > t0 + 1;      // O_1 holds something
+        const bool saw = mine && lim > t0 * kTile;  // some key of the piece
+        auto load = [&](int c, float(&o)[32]) {     // 32 columns of the row's sums
+          if (has) {
             tmem_ld32(to + 32 * c, o);
             tmem_wait_ld();
           }
-          if (mine) {
+          if (both) {
+            float o1[32];
+            tmem_ld32(to + 128 + 32 * c, o1);
+            tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t pk[4];
+            for (int i = 0; i < 32; ++i) o[i] = f0 * o[i] + f1 * o1[i];
+          }
+        };
+        if (slot < 0) {
+          const float inv = 1.f / l;
+          __nv_bfloat16* op = a.out + (w.row0 + rtok) * a.o_stride +
+                              ((long long)w.head * grp + r % grp) * kHeadDim;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            load(c, o);
+            if (mine) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                pk[k] = saw ? pack_bf16(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv) : 0u;
-              *reinterpret_cast<uint4*>(op + 32 * c + 8 * i) =
-                  make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              for (int i = 0; i < 4; ++i) {
+                uint32_t pk[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  pk[k] = saw ? pack_bf16(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv) : 0u;
+                *reinterpret_cast<uint4*>(op + 32 * c + 8 * i) =
+                    make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              }
             }
           }
-        }
-      } else {
-        // a row that saw nothing of the piece: (-inf, 0), its sums are not read
-        const int piece = 2 * blockIdx.x + slot;
-        float* po = p.ws.sums(piece) + (t * kRows + r) * kHeadDim;
+        } else {
+          // a row that saw nothing of the piece: (-inf, 0), its sums are not read
+          const int piece = 2 * blockIdx.x + slot;
+          float* po = p.ws.sums(piece) + (t * kRows + r) * kHeadDim;
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float o[32];
-          if (t1 > t0) {
-            tmem_ld32(to + 32 * c, o);
-            tmem_wait_ld();
-          }
-          if (saw) {
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            load(c, o);
+            if (saw) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<float4*>(po + 32 * c + 4 * i) =
-                  make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(po + 32 * c + 4 * i) =
+                    make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
           }
+          reinterpret_cast<float2*>(p.ws.stats(piece))[t * kRows + r] =
+              saw ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         }
-        reinterpret_cast<float2*>(p.ws.stats(piece))[t * kRows + r] =
-            saw ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+        if (twin) {
+          tc_fence_before();
+          mbar_arrive(&bars.twin_done);
+        }
         const int toks = min(w.toks - t * g.sub, g.sub);
-        if (toks > 0) {
+        if (slot >= 0 && toks > 0) {
           const long long out0 = w.row0 + t * g.sub;
           attn_join<4, 8>(
               p.ws, w.pieces, t, t * kRows, toks * grp, warp & 3, &sh.joining[t],
