@@ -42,7 +42,7 @@ constexpr int kWorks = 2;  // items handed out ahead
 struct Bars {
   uint64_t q_full[2], q_empty;
   uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t s_full[2], p_ready[2], o_full[2];
+  uint64_t s_full[2], p_ready[2][2], o_full[2];
   uint64_t work_full[kWorks], work_empty[kWorks];
   uint64_t twin_ready, twin_done;
   uint64_t drain;
@@ -124,6 +124,119 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+// One lane of a converged warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+// mbar_wait that also gives up when another role has.
+__device__ __forceinline__ bool mbar_wait_or(uint64_t* bar, uint32_t parity, volatile int* failed) {
+  for (uint32_t i = 0; i < (1u << 24); ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *failed) return false;
+  }
+  return false;
+}
+
+__device__ __forceinline__ float max3_nan(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+__device__ __forceinline__ float max_of(const float (&s)[4][32]) {
+  float m[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {  // four chains
+    m[c] = max3_nan(s[c][0], s[c][1], s[c][2]);
+#pragma unroll
+    for (int i = 3; i < 31; i += 2) m[c] = max3_nan(m[c], s[c][i], s[c][i + 1]);
+    m[c] = max3_nan(m[c], s[c][31], s[c][31]);
+  }
+  return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+}
+
+// Two fp32 values in one register pair.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+
+// 2^x of a finite pair, below 2^9 (from 2^-126 up; less gives 2^-126), on the FMA pipe: the
+// nearest integer n comes out of the sum with 1.5 2^23, and 2^(x - n) on [-1/2, 1/2] is a
+// cubic, fitted by reweighted least squares to a relative error of 7.5e-5 at most, a
+// fiftieth of the rounding to bf16 that follows.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  const float2 v = unpair(x);
+  const uint64_t y = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const uint64_t big = pair(12582912.f, 12582912.f), less = pair(-12582912.f, -12582912.f);
+  const uint64_t n = add2(y, big);
+  const uint64_t f = fma2(add2(n, less), pair(-1.f, -1.f), y);
+  uint64_t r = fma2(f, pair(0.0551716685f, 0.0551716685f), pair(0.242611125f, 0.242611125f));
+  r = fma2(r, f, pair(0.693260968f, 0.693260968f));
+  r = fma2(r, f, pair(0.999928057f, 0.999928057f));
+  const float2 p = unpair(r), k = unpair(n);
+  return pair(__int_as_float(__float_as_int(p.x) + (__float_as_int(k.x) << 23)),
+              __int_as_float(__float_as_int(p.y) + (__float_as_int(k.y) << 23)));
+}
+
+// P = 2^(scale s + shift) of a row into TMEM (bf16), each half of the keys announced; returns
+// the row's sum.  With kMixed a quarter of the exponentials go to the FMA pipe: 16 a clock is
+// what the special-function units of an SM give, which is just what the products take.
+constexpr int kMixEvery = 4;  // pairs
+template <bool kMixed>
+__device__ __forceinline__ float exponentials(const float (&s)[4][32], float scale, float shift,
+                                              uint32_t ts, uint64_t (&ready)[2]) {
+  const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t x = fma2(pair(s[c][2 * i], s[c][2 * i + 1]), scale2, shift2);
+      uint64_t y;
+      if (kMixed && i % kMixEvery == kMixEvery - 1) {
+        y = exp2_pair(x);
+      } else {
+        const float2 v = unpair(x);
+        y = pair(ex2(v.x), ex2(v.y));
+      }
+      sum[i & 1] = add2(sum[i & 1], y);
+      const float2 v = unpair(y);
+      pk[i] = pack_bf16(v.x, v.y);
+    }
+    tmem_st16(ts + 16 * c, pk);
+    if (c & 1) {
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&ready[c >> 1]);
+    }
+  }
+  const float2 v = unpair(add2(sum[0], sum[1]));
+  return v.x + v.y;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv, const TcArgs p) {
@@ -142,7 +255,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&b.q_full[t], 1);
       mbar_init(&b.s_full[t], 1);
-      mbar_init(&b.p_ready[t], 128);
+      mbar_init(&b.p_ready[t][0], 128);
+      mbar_init(&b.p_ready[t][1], 128);
       mbar_init(&b.o_full[t], 1);
     }
     mbar_init(&b.q_empty, 1);
@@ -275,130 +389,144 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 8) {
       // ------------------------------------------------------------------ products
-      if (lane == 0) {
-        constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false);
-        constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
-        uint32_t tile0 = 0;             // K / V tiles before this piece
-        uint32_t np0 = 0, np1 = 0;      // p_ready phases used
-        uint32_t nq0 = 0, nq1 = 0;      // q_full phases used
-        bool ok = true;
-        unsigned why = 0;
-        auto wait = [&](uint64_t* bar, uint32_t phase, unsigned err) {
-          if (!ok) return;
-          ok = mbar_wait(bar, phase & 1);
-          if (!ok) why = err;
-          if (*failed) ok = false;
-        };
-        auto scores = [&](int t, int qt, uint32_t entry) {  // S_t = Q_qt K^T
-          const uint32_t k = skv + entry % kStages * kTileBytes;
-          const uint32_t q = sq + qt * kTileBytes;
+      // The whole warp walks the tiles, so that addresses and descriptors stay in uniform
+      // registers; one elected lane issues.  (A single lane that did both took 100 cycles for
+      // each product, which last 64.)
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
+      const uint64_t qdesc = umma_desc_k(sq), kdesc = umma_desc_k(skv);
+      const uint64_t vdesc = umma_desc_mn(skv, kHalfBytes);
+      constexpr uint32_t kStep = kTileBytes >> 4;  // of a descriptor, to the next tile
+      const uint32_t td = __shfl_sync(0xffffffffu, tmem, 0);
+      uint32_t tile0 = 0;         // K / V tiles before this piece
+      uint32_t np0 = 0, np1 = 0;  // p_ready phases used
+      uint32_t nq0 = 0, nq1 = 0;  // q_full phases used
+      bool ok = true;
+      unsigned why = 0;
+      auto wait = [&](uint64_t* bar, uint32_t phase, unsigned err) {
+        if (!ok) return;
+        ok = __all_sync(0xffffffffu, mbar_wait_or(bar, phase & 1, failed));
+        if (!ok) why = err;
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+      };
+      auto wait_kv = [&](uint32_t entry) {
+        wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
+      };
+      auto scores = [&](int t, int qt, uint32_t entry) {  // S_t = Q_qt K^T
+        const uint64_t q = qdesc + qt * kStep, k = kdesc + entry % kStages * kStep;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const uint32_t off = (i >> 2) * kHalfBytes + (i & 3) * 32;
-            umma_bf16(tmem + 128 * t, umma_desc_k(q + off), umma_desc_k(k + off), idesc_s, i > 0);
+            const uint32_t off = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
+            umma_bf16(td + 128 * t, q + off, k + off, idesc_s, i > 0);
           }
           umma_commit(&bars.s_full[t]);
-        };
-        auto values = [&](int t, uint32_t entry, bool first) {  // O_t += P_t V
-          const uint32_t v = skv + entry % kStages * kTileBytes;
+        }
+      };
+      // O_t += P_t V, in two halves of the keys as P's are written
+      auto values = [&](int t, uint32_t entry, bool first) {
+        const uint64_t v = vdesc + entry % kStages * kStep;
+        const uint32_t phase = t ? np1++ : np0++;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            umma_bf16_tmem_a(tmem + 256 + 128 * t, tmem + 128 * t + 8 * i,
-                             umma_desc_mn(v + i * 2048, kHalfBytes), idesc_o, !first || i > 0);
-        };
-        for (uint32_t n = 0; ok; ++n) {
-          wait(&bars.work_full[n % kWorks], n / kWorks, kErrLoad);
-          if (!ok || !sh.work[n % kWorks].live) break;
-          const int t0 = sh.work[n % kWorks].t0, t1 = sh.work[n % kWorks].t1;
-          const int end0 = sh.work[n % kWorks].end[0], end1 = sh.work[n % kWorks].end[1];
-          const bool twin = sh.work[n % kWorks].twin;
-          mbar_arrive(&bars.work_empty[n % kWorks]);
-          if (t1 <= t0) continue;
-          if (twin) {
-            // key tile j goes to half (j - t0) % 2; its scores are taken two tiles ahead
-            wait(&bars.q_full[0], nq0++, kErrLoad);
-            auto ahead = [&](int j) {
-              const uint32_t e = 2 * (tile0 + j - t0);
-              wait(&bars.kv_full[e % kStages], e / kStages, kErrLoad);
-              if (!ok) return;
-              tc_fence_after();
-              scores((j - t0) & 1, 0, e);
-              umma_commit(&bars.kv_empty[e % kStages]);
-              if (j + 1 == t1) umma_commit(&bars.q_empty);
-            };
-            ahead(t0);
-            if (t0 + 1 < t1) ahead(t0 + 1);
-            for (int j = t0; j < t1 && ok; ++j) {
-              const uint32_t e = 2 * (tile0 + j - t0) + 1;
-              const int t = (j - t0) & 1;
-              wait(&bars.kv_full[e % kStages], e / kStages, kErrLoad);
-              wait(&bars.p_ready[t], t ? np1++ : np0++, kErrTensor);
-              if (!ok) break;
-              tc_fence_after();
-              values(t, e, j < t0 + 2);
-              umma_commit(&bars.kv_empty[e % kStages]);
-              if (j + 2 < t1) ahead(j + 2);
-              else umma_commit(&bars.o_full[t]);
-            }
-            tile0 += t1 - t0;
-            continue;
+        for (int h = 0; h < 2; ++h) {
+          wait(&bars.p_ready[t][h], phase, kErrTensor);
+          tc_fence_after();
+          if (ok && elect_one()) {
+#pragma unroll
+            for (int i = 4 * h; i < 4 * h + 4; ++i)
+              umma_bf16_tmem_a(td + 256 + 128 * t, td + 128 * t + 8 * i, v + i * (2048 >> 4),
+                               idesc_o, !first || i > 0);
           }
-          // the row tile that holds the block's last token needs every key tile: it comes last
-          // and releases what both have read
-          const int last = end1 == t1 ? 1 : 0;
-          uint32_t entry = 2 * tile0;
-          wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
-          auto begin = [&](int t) {  // scores of tile j into S_t; K and, at the end, Q released
-            scores(t, t, entry);
-            if (t == last) umma_commit(&bars.kv_empty[entry % kStages]);
+        }
+      };
+      for (uint32_t n = 0; ok; ++n) {
+        wait(&bars.work_full[n % kWorks], n / kWorks, kErrLoad);
+        const Work& w = sh.work[n % kWorks];
+        if (!ok || !w.live) break;
+        const int t0 = __shfl_sync(0xffffffffu, w.t0, 0), t1 = __shfl_sync(0xffffffffu, w.t1, 0);
+        const int end0 = __shfl_sync(0xffffffffu, w.end[0], 0);
+        const int end1 = __shfl_sync(0xffffffffu, w.end[1], 0);
+        const bool twin = __shfl_sync(0xffffffffu, (int)w.twin, 0) != 0;
+        if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
+        if (t1 <= t0) continue;
+        if (twin) {
+          // key tile j goes to half (j - t0) % 2; its scores are taken two tiles ahead
+          wait(&bars.q_full[0], nq0++, kErrLoad);
+          auto ahead = [&](int j) {
+            const uint32_t e = 2 * (tile0 + j - t0);
+            wait_kv(e);
+            if (!ok) return;
+            scores((j - t0) & 1, 0, e);
+            commit(&bars.kv_empty[e % kStages]);
+            if (j + 1 == t1) commit(&bars.q_empty);
           };
-          if (end0 > t0) {
-            wait(&bars.q_full[0], nq0++, kErrLoad);
-            if (!ok) break;
-            tc_fence_after();
-            begin(0);
-          }
-          if (end1 > t0) {
-            wait(&bars.q_full[1], nq1++, kErrLoad);
-            if (!ok) break;
-            tc_fence_after();
-            begin(1);
-          }
-          if (t0 + 1 == t1) umma_commit(&bars.q_empty);
+          ahead(t0);
+          if (t0 + 1 < t1) ahead(t0 + 1);
           for (int j = t0; j < t1 && ok; ++j) {
-            const uint32_t ve = entry + 1;  // V of tile j; the K of tile j + 1 comes behind it
-            entry += 2;
-            wait(&bars.kv_full[ve % kStages], ve / kStages, kErrLoad);
-            if (j + 1 < t1) wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
-            if (j < end0) {
-              wait(&bars.p_ready[0], np0++, kErrTensor);
-              if (!ok) break;
-              tc_fence_after();
-              values(0, ve, j == t0);
-              if (last == 0) umma_commit(&bars.kv_empty[ve % kStages]);
-              if (j + 1 < end0) begin(0);
-              else umma_commit(&bars.o_full[0]);
-            }
-            if (j < end1) {
-              wait(&bars.p_ready[1], np1++, kErrTensor);
-              if (!ok) break;
-              tc_fence_after();
-              values(1, ve, j == t0);
-              if (last == 1) umma_commit(&bars.kv_empty[ve % kStages]);
-              if (j + 1 < end1) begin(1);
-              else umma_commit(&bars.o_full[1]);
-            }
-            if (j + 2 == t1) umma_commit(&bars.q_empty);
+            const uint32_t e = 2 * (tile0 + j - t0) + 1;
+            const int t = (j - t0) & 1;
+            wait_kv(e);
+            values(t, e, j < t0 + 2);
+            if (!ok) break;
+            commit(&bars.kv_empty[e % kStages]);
+            if (j + 2 < t1) ahead(j + 2);
+            else commit(&bars.o_full[t]);
           }
           tile0 += t1 - t0;
+          continue;
         }
-        if (!ok) {
-          *failed = 1;
-          if (why) atomicOr(&g_attn_error, why);
+        // the row tile that holds the block's last token needs every key tile: it comes last
+        // and releases what both have read
+        const int last = end1 == t1 ? 1 : 0;
+        uint32_t entry = 2 * tile0;
+        auto begin = [&](int t) {  // scores of the K tile at `entry`, released by the last
+          scores(t, t, entry);
+          if (t == last) commit(&bars.kv_empty[entry % kStages]);
+        };
+        wait_kv(entry);
+        if (end0 > t0) {
+          wait(&bars.q_full[0], nq0++, kErrLoad);
+          if (!ok) break;
+          begin(0);
         }
-        umma_commit(&bars.drain);  // nothing is in flight when the block ends
-        mbar_wait(&bars.drain, 0);
+        if (end1 > t0) {
+          wait(&bars.q_full[1], nq1++, kErrLoad);
+          if (!ok) break;
+          begin(1);
+        }
+        if (t0 + 1 == t1) commit(&bars.q_empty);
+        for (int j = t0; j < t1 && ok; ++j) {
+          const uint32_t ve = entry + 1;  // V of tile j; the K of tile j + 1 comes behind it
+          entry += 2;
+          wait_kv(ve);
+          if (j + 1 < t1) wait_kv(entry);
+          if (j < end0) {
+            values(0, ve, j == t0);
+            if (!ok) break;
+            if (last == 0) commit(&bars.kv_empty[ve % kStages]);
+            if (j + 1 < end0) begin(0);
+            else commit(&bars.o_full[0]);
+          }
+          if (j < end1) {
+            values(1, ve, j == t0);
+            if (!ok) break;
+            if (last == 1) commit(&bars.kv_empty[ve % kStages]);
+            if (j + 1 < end1) begin(1);
+            else commit(&bars.o_full[1]);
+          }
+          if (j + 2 == t1) commit(&bars.q_empty);
+        }
+        tile0 += t1 - t0;
       }
+      if (!ok) {
+        *failed = 1;
+        if (why && lane == 0) atomicOr(&g_attn_error, why);
+      }
+      commit(&bars.drain);  // nothing is in flight when the block ends
+      mbar_wait(&bars.drain, 0);
     }
   } else {
     // ------------------------------------------------------------------ softmax
@@ -440,12 +568,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) s[c][i] = 32 * c + i < vis ? s[c][i] : -INFINITY;
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, s[c][i]);
-        mx *= a.scale_log2;  // scale > 0
+        float mx = max_of(s);  // NaN if any is
+        mx *= a.scale_log2;    // scale > 0
         const bool raise = mx > m + kRaise;  // always for the first finite score
         if (__any_sync(0xffffffffu, raise)) {
           const float m2 = raise ? mx : m;
@@ -464,21 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           m = m2;
         }
-        const float mm = m == -INFINITY ? 0.f : m;
-        float sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float x = ex2(fmaf(s[c][2 * i], a.scale_log2, -mm));
-            const float y = ex2(fmaf(s[c][2 * i + 1], a.scale_log2, -mm));
-            sum += x + y;
-            pk[i] = pack_bf16(x, y);
-          }
-          tmem_st16(ts + 16 * c, pk);
-        }
-        l += sum;
         if ((j + 1) * kTile > kv_len) {  // rows of V behind the last key
           const uint32_t entry = 2 * (tile0 + j - t0) + 1;
           ok = __all_sync(0xffffffffu,
@@ -493,9 +602,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bars.p_ready[t]);
+        const float mm = m == -INFINITY ? 0.f : m;
+        if (__any_sync(0xffffffffu, vis < kTile || !(fabsf(mx) < INFINITY)))
+          l += exponentials<false>(s, a.scale_log2, -mm, ts, bars.p_ready[t]);
+        else
+          l += exponentials<true>(s, a.scale_log2, -mm, ts, bars.p_ready[t]);
         if (!ok) break;
       }
       if (t1 > jb && ok)
