@@ -19,7 +19,7 @@ namespace gdn {
 // of the one its range ends inside (slot 1)
 constexpr int kAttnSlots = 2;
 constexpr int kAttnTile = 128;      // keys per tile
-constexpr int kAttnMaxParts = 160;  // CTAs that share the work (one per SM)
+constexpr int kAttnMaxParts = 152;  // CTAs that share the work (one per SM)
 
 struct AttnGrid {
   int block;     // query tokens per item

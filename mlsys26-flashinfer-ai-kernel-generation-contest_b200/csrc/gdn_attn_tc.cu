@@ -29,6 +29,7 @@ using namespace sm100;
 
 constexpr int kRows = 128;             // rows of a tile
 constexpr int kTile = kAttnTile;       // keys of a tile
+constexpr int kPart = 64;              // keys that a row's scores are taken for at once
 constexpr int kStages = 5;             // K / V ring
 constexpr int kHalfBytes = 128 * 128;  // 64 columns of 128 rows, 128-byte swizzle
 constexpr int kTileBytes = 2 * kHalfBytes;
@@ -42,10 +43,10 @@ constexpr int kWorks = 2;  // items handed out ahead
 struct Bars {
   uint64_t q_full[2], q_empty;
   uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t s_full[2], p_ready[2][2], o_full[2];
+  uint64_t s_full[2][2], p_ready[2][2], pv_done[2], o_full[2];
   uint64_t work_full[kWorks], work_empty[kWorks];
   uint64_t twin_ready, twin_done;
-  uint64_t drain;
+  uint64_t drain[2];
 };
 // One piece of an item, for all roles.
 struct Work {
@@ -148,14 +149,16 @@ __device__ __forceinline__ float max3_nan(float x, float y, float z) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
-__device__ __forceinline__ float max_of(const float (&s)[4][32]) {
+__device__ __forceinline__ float max_of(const float (&s)[2][32]) {  // NaN if any is
   float m[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {  // four chains
-    m[c] = max3_nan(s[c][0], s[c][1], s[c][2]);
+  for (int k = 0; k < 4; ++k) {  // four chains
+    const float(&x)[32] = s[k >> 1];
+    const int o = 16 * (k & 1);
+    m[k] = max3_nan(x[o], x[o + 1], x[o + 2]);
 #pragma unroll
-    for (int i = 3; i < 31; i += 2) m[c] = max3_nan(m[c], s[c][i], s[c][i + 1]);
-    m[c] = max3_nan(m[c], s[c][31], s[c][31]);
+    for (int i = 3; i < 15; i += 2) m[k] = max3_nan(m[k], x[o + i], x[o + i + 1]);
+    m[k] = max3_nan(m[k], x[o + 15], x[o + 15]);
   }
   return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
 }
@@ -200,17 +203,17 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
               __int_as_float(__float_as_int(p.y) + (__float_as_int(k.y) << 23)));
 }
 
-// P = 2^(scale s + shift) of a row into TMEM (bf16), each half of the keys announced; returns
-// the row's sum.  With kMixed a quarter of the exponentials go to the FMA pipe: 16 a clock is
-// what the special-function units of an SM give, which is just what the products take.
+// P = 2^(scale s + shift) of a row's part into TMEM (bf16, over the scores); returns the sum.
+// With kMixed a quarter of the exponentials go to the FMA pipe: 16 a clock is what the
+// special-function units of an SM give, which is just what the products take.
 constexpr int kMixEvery = 4;  // pairs
 template <bool kMixed>
-__device__ __forceinline__ float exponentials(const float (&s)[4][32], float scale, float shift,
-                                              uint32_t ts, uint64_t (&ready)[2]) {
+__device__ __forceinline__ float exponentials(const float (&s)[2][32], float scale, float shift,
+                                              uint32_t ts) {
   const uint64_t scale2 = pair(scale, scale), shift2 = pair(shift, shift);
   uint64_t sum[2] = {0, 0};
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
+  for (int c = 0; c < 2; ++c) {
     uint32_t pk[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -227,11 +230,6 @@ __device__ __forceinline__ float exponentials(const float (&s)[4][32], float sca
       pk[i] = pack_bf16(v.x, v.y);
     }
     tmem_st16(ts + 16 * c, pk);
-    if (c & 1) {
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&ready[c >> 1]);
-    }
   }
   const float2 v = unpair(add2(sum[0], sum[1]));
   return v.x + v.y;
@@ -254,23 +252,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     Bars& b = sh.bars;
     for (int t = 0; t < 2; ++t) {
       mbar_init(&b.q_full[t], 1);
-      mbar_init(&b.s_full[t], 1);
-      mbar_init(&b.p_ready[t][0], 128);
-      mbar_init(&b.p_ready[t][1], 128);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&b.s_full[t][h], 1);
+        mbar_init(&b.p_ready[t][h], 4);  // a warp arrives as one
+      }
+      mbar_init(&b.pv_done[t], 1);
+      mbar_init(&b.drain[t], 1);
       mbar_init(&b.o_full[t], 1);
     }
-    mbar_init(&b.q_empty, 1);
+    mbar_init(&b.q_empty, 2);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&b.kv_full[i], 1);
-      mbar_init(&b.kv_empty[i], 1);
+      mbar_init(&b.kv_empty[i], 2);  // the two issuing warps
     }
     for (int i = 0; i < kWorks; ++i) {
       mbar_init(&b.work_full[i], 1);
-      mbar_init(&b.work_empty[i], 10);  // loader, issuer, eight softmax warps
+      mbar_init(&b.work_empty[i], 11);  // loader, two issuers, eight softmax warps
     }
-    mbar_init(&b.twin_ready, 128);
-    mbar_init(&b.twin_done, 128);
-    mbar_init(&b.drain, 1);
+    mbar_init(&b.twin_ready, 4);
+    mbar_init(&b.twin_done, 4);
     fence_mbar_init();
     sh.failed = 0;
     tma_prefetch_desc(&mq);
@@ -387,19 +387,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = ring > kStages ? ring - kStages : 0; i < ring; ++i)
           mbar_wait(&bars.kv_full[i % kStages], (i / kStages) & 1, 1u << 20);
       }
-    } else if (warp == 8) {
+    } else if (warp == 8 || warp == 11) {
       // ------------------------------------------------------------------ products
-      // The whole warp walks the tiles, so that addresses and descriptors stay in uniform
-      // registers; one elected lane issues.  (A single lane that did both took 100 cycles for
-      // each product, which last 64.)
-      constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, false, false);
+      // A warp for each row tile (or, for twins, each half of the key tiles).  The whole warp
+      // walks the tiles, so that addresses and descriptors stay in uniform registers; one
+      // elected lane issues.  (A single lane that did both took 100 cycles for each product,
+      // which last 64.)
+      const int t = warp == 8 ? 0 : 1;
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPart, false, false);
       constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
       const uint64_t qdesc = umma_desc_k(sq), kdesc = umma_desc_k(skv);
       const uint64_t vdesc = umma_desc_mn(skv, kHalfBytes);
       constexpr uint32_t kStep = kTileBytes >> 4;  // of a descriptor, to the next tile
-      const uint32_t td = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t td = __shfl_sync(0xffffffffu, tmem, 0) + 128 * t;
       uint32_t tile0 = 0;         // K / V tiles before this piece
-      uint32_t np0 = 0, np1 = 0;  // p_ready phases used
+      uint32_t np = 0;            // p_ready phases used
       uint32_t nq0 = 0, nq1 = 0;  // q_full phases used
       bool ok = true;
       unsigned why = 0;
@@ -414,32 +416,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto wait_kv = [&](uint32_t entry) {
         wait(&bars.kv_full[entry % kStages], entry / kStages, kErrLoad);
       };
-      auto scores = [&](int t, int qt, uint32_t entry) {  // S_t = Q_qt K^T
-        const uint64_t q = qdesc + qt * kStep, k = kdesc + entry % kStages * kStep;
+      // this warp has no use for a ring entry (arrived only when it is there: in step)
+      auto skip_kv = [&](uint32_t entry) {
+        wait_kv(entry);
+        if (ok && elect_one()) mbar_arrive(&bars.kv_empty[entry % kStages]);
+      };
+      auto scores = [&](uint64_t q, uint32_t entry, int h) {  // S_h = Q K^T, keys 64 h ..
+        const uint64_t k = kdesc + entry % kStages * kStep + h * (kPart * 128 >> 4);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const uint32_t off = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
-            umma_bf16(td + 128 * t, q + off, k + off, idesc_s, i > 0);
+            umma_bf16(td + kPart * h, q + off, k + off, idesc_s, i > 0);
           }
-          umma_commit(&bars.s_full[t]);
+          umma_commit(&bars.s_full[t][h]);
         }
       };
-      // O_t += P_t V, in two halves of the keys as P's are written
-      auto values = [&](int t, uint32_t entry, bool first) {
-        const uint64_t v = vdesc + entry % kStages * kStep;
-        const uint32_t phase = t ? np1++ : np0++;
+      auto values = [&](uint32_t entry, int h, bool first) {  // O += P_h V, keys 64 h ..
+        const uint64_t v = vdesc + entry % kStages * kStep + h * (kPart * 128 >> 4);
+        wait(&bars.p_ready[t][h], np, kErrTensor);
+        tc_fence_after();
+        if (ok && elect_one()) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          wait(&bars.p_ready[t][h], phase, kErrTensor);
-          tc_fence_after();
-          if (ok && elect_one()) {
-#pragma unroll
-            for (int i = 4 * h; i < 4 * h + 4; ++i)
-              umma_bf16_tmem_a(td + 256 + 128 * t, td + 128 * t + 8 * i, v + i * (2048 >> 4),
-                               idesc_o, !first || i > 0);
-          }
+          for (int i = 0; i < kPart / 16; ++i)
+            umma_bf16_tmem_a(td + 256, td + kPart * h + 8 * i, v + i * (2048 >> 4), idesc_o,
+                             !first || i > 0);
+          umma_commit(&bars.pv_done[t]);
         }
       };
       for (uint32_t n = 0; ok; ++n) {
@@ -452,81 +455,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool twin = __shfl_sync(0xffffffffu, (int)w.twin, 0) != 0;
         if (lane == 0) mbar_arrive(&bars.work_empty[n % kWorks]);
         if (t1 <= t0) continue;
-        if (twin) {
-          // key tile j goes to half (j - t0) % 2; its scores are taken two tiles ahead
-          wait(&bars.q_full[0], nq0++, kErrLoad);
-          auto ahead = [&](int j) {
-            const uint32_t e = 2 * (tile0 + j - t0);
-            wait_kv(e);
-            if (!ok) return;
-            scores((j - t0) & 1, 0, e);
-            commit(&bars.kv_empty[e % kStages]);
-            if (j + 1 == t1) commit(&bars.q_empty);
-          };
-          ahead(t0);
-          if (t0 + 1 < t1) ahead(t0 + 1);
-          for (int j = t0; j < t1 && ok; ++j) {
-            const uint32_t e = 2 * (tile0 + j - t0) + 1;
-            const int t = (j - t0) & 1;
-            wait_kv(e);
-            values(t, e, j < t0 + 2);
-            if (!ok) break;
-            commit(&bars.kv_empty[e % kStages]);
-            if (j + 2 < t1) ahead(j + 2);
-            else commit(&bars.o_full[t]);
+        if (end0 > t0) wait(&bars.q_full[0], nq0++, kErrLoad);
+        if (end1 > t0) wait(&bars.q_full[1], nq1++, kErrLoad);
+        // this warp's key tiles: first, first + step, .. below end
+        const int first = t0 + (twin ? t : 0), step = twin ? 2 : 1;
+        const int end = twin ? t1 : (t ? end1 : end0);
+        const uint64_t q = qdesc + (twin ? 0 : t) * kStep;
+        auto entry_of = [&](int j) { return 2 * (tile0 + j - t0); };
+        int at = t0;  // ring entries of tiles before `at` are used or skipped
+        auto skip_to = [&](int j) {
+          for (; at < j && ok; ++at) {
+            skip_kv(entry_of(at));
+            skip_kv(entry_of(at) + 1);
           }
-          tile0 += t1 - t0;
-          continue;
-        }
-        // the row tile that holds the block's last token needs every key tile: it comes last
-        // and releases what both have read
-        const int last = end1 == t1 ? 1 : 0;
-        uint32_t entry = 2 * tile0;
-        auto begin = [&](int t) {  // scores of the K tile at `entry`, released by the last
-          scores(t, t, entry);
-          if (t == last) commit(&bars.kv_empty[entry % kStages]);
         };
-        wait_kv(entry);
-        if (end0 > t0) {
-          wait(&bars.q_full[0], nq0++, kErrLoad);
+        if (first < end) {
+          skip_to(first);
+          uint32_t k = entry_of(first);
+          wait_kv(k);
           if (!ok) break;
-          begin(0);
-        }
-        if (end1 > t0) {
-          wait(&bars.q_full[1], nq1++, kErrLoad);
-          if (!ok) break;
-          begin(1);
-        }
-        if (t0 + 1 == t1) commit(&bars.q_empty);
-        for (int j = t0; j < t1 && ok; ++j) {
-          const uint32_t ve = entry + 1;  // V of tile j; the K of tile j + 1 comes behind it
-          entry += 2;
-          wait_kv(ve);
-          if (j + 1 < t1) wait_kv(entry);
-          if (j < end0) {
-            values(0, ve, j == t0);
+          scores(q, k, 0);
+          scores(q, k, 1);
+          commit(&bars.kv_empty[k % kStages]);
+          if (first + step >= end) commit(&bars.q_empty);
+          for (int j = first; j < end && ok; j += step) {
+            const uint32_t v = k + 1;
+            const bool more = j + step < end;
+            wait_kv(v);
+            values(v, 0, j == first);
+            if (more) {
+              at = j + 1;
+              skip_to(j + step);
+              k = entry_of(j + step);
+              wait_kv(k);
+              if (!ok) break;
+              scores(q, k, 0);
+            }
+            values(v, 1, false);
+            ++np;
             if (!ok) break;
-            if (last == 0) commit(&bars.kv_empty[ve % kStages]);
-            if (j + 1 < end0) begin(0);
-            else commit(&bars.o_full[0]);
+            commit(&bars.kv_empty[v % kStages]);
+            if (more) {
+              scores(q, k, 1);
+              commit(&bars.kv_empty[k % kStages]);
+              if (j + 2 * step >= end) commit(&bars.q_empty);
+            } else {
+              commit(&bars.o_full[t]);
+            }
+            at = j + 1;
           }
-          if (j < end1) {
-            values(1, ve, j == t0);
-            if (!ok) break;
-            if (last == 1) commit(&bars.kv_empty[ve % kStages]);
-            if (j + 1 < end1) begin(1);
-            else commit(&bars.o_full[1]);
-          }
-          if (j + 2 == t1) commit(&bars.q_empty);
+        } else if (ok) {
+          commit(&bars.q_empty);
         }
+        skip_to(t1);
         tile0 += t1 - t0;
       }
       if (!ok) {
         *failed = 1;
         if (why && lane == 0) atomicOr(&g_attn_error, why);
       }
-      commit(&bars.drain);  // nothing is in flight when the block ends
-      mbar_wait(&bars.drain, 0);
+      commit(&bars.drain[t]);  // nothing is in flight when the block ends
+      mbar_wait(&bars.drain[t], 0);
     }
   } else {
     // ------------------------------------------------------------------ softmax
@@ -535,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = tid & 127;        // row
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane field: 32 (warp % 4)
     const uint32_t ts = tmem + 128 * t + lanes, to = tmem + 256 + 128 * t + lanes;
-    uint32_t ns = 0, no = 0, nt = 0, tile0 = 0;
+    uint32_t ns = 0, no = 0, nt = 0, npv = 0, tile0 = 0;
     bool ok = true;
     for (uint32_t n = 0;; ++n) {
       if (!__all_sync(0xffffffffu, mbar_wait(&bars.work_full[n % kWorks], n / kWorks & 1))) ok = false;
@@ -553,41 +542,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int kv_len = w.kv_len, t0 = w.t0, t1 = w.end[rt];
       const int jb = twin ? t0 + t : t0, step = twin ? 2 : 1;  // this half's key tiles
       float m = -INFINITY, l = 0.f;  // m in log2 units
-      for (int j = jb; j < t1; j += step) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], ns++ & 1));
-        if (!ok) break;
-        tc_fence_after();
-        float s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
-        tmem_wait_ld();
-        const int vis = lim - j * kTile;  // visible columns of this tile
-        if (__any_sync(0xffffffffu, vis < kTile)) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[c][i] = 32 * c + i < vis ? s[c][i] : -INFINITY;
-        }
-        float mx = max_of(s);  // NaN if any is
-        mx *= a.scale_log2;    // scale > 0
-        const bool raise = mx > m + kRaise;  // always for the first finite score
-        if (__any_sync(0xffffffffu, raise)) {
-          const float m2 = raise ? mx : m;
-          const float f = m == -INFINITY ? 0.f : ex2(m - m2);
-          l *= f;
-          if (j > jb) {  // O holds earlier tiles: their product is complete (s_full came after)
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {  // 16 columns at a time: few registers, rare
-              uint32_t o[16];
-              tmem_ld16(to + 16 * c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st16(to + 16 * c, o);
-            }
-          }
-          m = m2;
-        }
+      uint32_t parts = 0;            // of the piece so far
+      for (int j = jb; j < t1 && ok; j += step) {
         if ((j + 1) * kTile > kv_len) {  // rows of V behind the last key
           const uint32_t entry = 2 * (tile0 + j - t0) + 1;
           ok = __all_sync(0xffffffffu,
@@ -602,13 +558,60 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_proxy_async();
         }
-        const float mm = m == -INFINITY ? 0.f : m;
-        if (__any_sync(0xffffffffu, vis < kTile || !(fabsf(mx) < INFINITY)))
-          l += exponentials<false>(s, a.scale_log2, -mm, ts, bars.p_ready[t]);
-        else
-          l += exponentials<true>(s, a.scale_log2, -mm, ts, bars.p_ready[t]);
-        if (!ok) break;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t][h], ns & 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t tp = ts + kPart * h;
+          float s[2][32];
+          tmem_ld32(tp, s[0]);
+          tmem_ld32(tp + 32, s[1]);
+          tmem_wait_ld();
+          const int vis = lim - j * kTile - h * kPart;  // visible columns
+          const bool masked = __any_sync(0xffffffffu, vis < kPart);
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              s[0][i] = i < vis ? s[0][i] : -INFINITY;
+              s[1][i] = 32 + i < vis ? s[1][i] : -INFINITY;
+            }
+          }
+          const float mx = max_of(s) * a.scale_log2;  // scale > 0
+          const bool raise = mx > m + kRaise;         // always for the first finite score
+          if (__any_sync(0xffffffffu, raise)) {
+            const float m2 = raise ? mx : m;
+            const float f = m == -INFINITY ? 0.f : ex2(m - m2);
+            l *= f;
+            if (parts > 0) {  // O holds earlier parts: once their product is complete
+              ok = __all_sync(0xffffffffu, mbar_wait(&bars.pv_done[t], (npv + parts - 1) & 1));
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < 8; ++c) {  // 16 columns at a time: few registers, rare
+                uint32_t o[16];
+                tmem_ld16(to + 16 * c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st16(to + 16 * c, o);
+              }
+            }
+            m = m2;
+          }
+          const float mm = m == -INFINITY ? 0.f : m;
+          if (masked || __any_sync(0xffffffffu, !(fabsf(mx) < INFINITY)))
+            l += exponentials<false>(s, a.scale_log2, -mm, tp);
+          else
+            l += exponentials<true>(s, a.scale_log2, -mm, tp);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.p_ready[t][h]);
+          ++parts;
+        }
+        ++ns;
       }
+      npv += parts;
       if (t1 > jb && ok)
         ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_full[t], no++ & 1));
       if (group_or(1 + t, 128, !ok)) {
@@ -621,7 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (twin && t == 1) {      // the first half reads this half's rows and finishes them
         sh.twin[r] = has ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
         tc_fence_before();
-        mbar_arrive(&bars.twin_ready);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.twin_ready);
         if (!__all_sync(0xffffffffu, mbar_wait(&bars.twin_done, nt++ & 1))) ok = false;
       } else {
         float f0 = 1.f, f1 = 0.f;  // weights of O_t and, for twins, of O_1
@@ -690,7 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (twin) {
           tc_fence_before();
-          mbar_arrive(&bars.twin_done);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.twin_done);
         }
         const int toks = min(w.toks - t * g.sub, g.sub);
         if (slot >= 0 && toks > 0) {
