@@ -252,79 +252,82 @@ __device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& l
   if (lane == 0) out->count = count;
 }
 
-// Joins `count` <= kAttnFan pieces list[0], list[step], .. of the rows [row0, row0 + rows):
-// kWarps warps, R rows of each at a time (loads of all of them in flight).  Every row goes
-// to out(row, lane's four columns, maximum, sum).
-template <int kWarps, int R, typename Out>
+// Joins `count` <= kAttnFan pieces list[0], list[step], .. of the rows [row0, row0 + rows),
+// by kWarps warps together (rows <= 32 kWarps).  First a thread takes a row's statistics and
+// leaves the pieces' weights in `weights` (kAttnFan x rows floats of shared memory), then a
+// warp takes R rows and U pieces at a time, all their loads in flight.  stat(row, maximum,
+// sum) gives what the row's weights are multiplied with, out(row, lane's four columns) gets
+// the weighted sums.
+template <int kWarps, int R, int U, typename Sync, typename Stat, typename Out>
 __device__ __forceinline__ void attn_merge(const AttnPartials& ws, const short* list, int step,
-                                           int count, int row0, int rows, int warp, Out&& out) {
-  constexpr int kPer = 32 / R, kRounds = kAttnFan / kPer;
-  const int lane = threadIdx.x & 31;
-  const int jl = lane / kPer, il = lane % kPer;  // the row and piece whose weight the lane has
-  for (int r = warp * R; r < rows; r += kWarps * R) {
-    float2 ml[kRounds];
-    float M = -INFINITY, l = 0.f, f[kRounds];
+                                           int count, int row0, int rows, int warp,
+                                           float* weights, Sync&& sync, Stat&& stat, Out&& out) {
+  const int lane = threadIdx.x & 31, r = warp * 32 + lane;
+  if (r < rows) {
+    float2 ml[kAttnFan];
+    float M = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
-      const int i = k * kPer + il;
-      ml[k] = make_float2(-INFINITY, 0.f);
-      if (i < count && r + jl < rows)
-        ml[k] = __ldcg(reinterpret_cast<const float2*>(ws.stats(list[i * step])) + row0 + r + jl);
-      if (ml[k].y != 0.f) M = fmaxf(M, ml[k].x);  // sum 0: the row saw nothing of the piece
+    for (int i = 0; i < kAttnFan; ++i)
+      ml[i] = i < count
+                  ? __ldcg(reinterpret_cast<const float2*>(ws.stats(list[i * step])) + row0 + r)
+                  : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int i = 0; i < kAttnFan; ++i)
+      if (ml[i].y != 0.f) M = fmaxf(M, ml[i].x);  // sum 0: the row saw nothing of the piece
+#pragma unroll
+    for (int i = 0; i < kAttnFan; ++i) {
+      ml[i].x = ml[i].y == 0.f ? 0.f : exp2f(ml[i].x - M);
+      l += ml[i].y == 0.f ? 0.f : ml[i].x * ml[i].y;
     }
+    const float f = stat(row0 + r, M, l);
 #pragma unroll
-    for (int w = 1; w < kPer; w <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
-#pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
-      f[k] = ml[k].y == 0.f ? 0.f : exp2f(ml[k].x - M);
-      l += ml[k].y == 0.f ? 0.f : f[k] * ml[k].y;
-    }
-#pragma unroll
-    for (int w = 1; w < kPer; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+    for (int i = 0; i < kAttnFan; ++i)
+      if (i < count) weights[i * rows + r] = ml[i].y == 0.f ? 0.f : ml[i].x * f;
+  }
+  sync();
+  for (int r0 = warp * R; r0 < rows; r0 += kWarps * R) {
     float4 o[R];
 #pragma unroll
     for (int j = 0; j < R; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < count; i0 += U) {
+      float4 x[U][R];
+      float w[U][R];
 #pragma unroll
-    for (int k = 0; k < kRounds; ++k) {
-#pragma unroll(R > 2 ? 2 : 8)  // loads of 16 rows in flight
-      for (int i = 0; i < kPer; ++i) {
-        if (k * kPer + i >= count) break;
-        const float* src = ws.sums(list[(k * kPer + i) * step]) +
-                           (long long)(row0 + r) * kHeadDim + 4 * lane;
-        float4 x[R];
-        float w[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-          w[j] = __shfl_sync(0xffffffffu, f[k], j * kPer + i);
-          x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (w[j] != 0.f) x[j] = __ldcg(reinterpret_cast<const float4*>(src + j * kHeadDim));
-        }
+      for (int i = 0; i < U; ++i) {
+        const bool there = i0 + i < count;
+        const float* src = ws.sums(list[(there ? i0 + i : 0) * step]) +
+                           (long long)(row0 + r0) * kHeadDim + 4 * lane;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-          o[j].x = fmaf(w[j], x[j].x, o[j].x);
-          o[j].y = fmaf(w[j], x[j].y, o[j].y);
-          o[j].z = fmaf(w[j], x[j].z, o[j].z);
-          o[j].w = fmaf(w[j], x[j].w, o[j].w);
+          w[i][j] = there && r0 + j < rows ? weights[(i0 + i) * rows + r0 + j] : 0.f;
+          x[i][j] = w[i][j] != 0.f ? __ldcg(reinterpret_cast<const float4*>(src + j * kHeadDim))
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          o[j].x = fmaf(w[i][j], x[i][j].x, o[j].x);
+          o[j].y = fmaf(w[i][j], x[i][j].y, o[j].y);
+          o[j].z = fmaf(w[i][j], x[i][j].z, o[j].z);
+          o[j].w = fmaf(w[i][j], x[i][j].w, o[j].w);
+        }
     }
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const float Mj = __shfl_sync(0xffffffffu, M, j * kPer);
-      const float lj = __shfl_sync(0xffffffffu, l, j * kPer);
-      if (r + j < rows) out(row0 + r + j, o[j], Mj, lj);
-    }
+    for (int j = 0; j < R; ++j)
+      if (r0 + j < rows) out(row0 + r0 + j, o[j]);
   }
 }
 
 // After a piece's partial result is written: by the kWarps warps that wrote the rows [row0,
 // row0 + rows) (row tile `tile`) together, `sync` their barrier, `flag` an int of theirs in
-// shared memory.  The last CTA of an item to come here writes its output through
-// store(row, four columns).
-template <int kWarps, int R, typename Sync, typename Store>
+// shared memory, `weights` kAttnFan x rows floats.  The last CTA of an item to come here
+// writes its output through store(row, four columns).
+template <int kWarps, int R, int U, typename Sync, typename Store>
 __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPieces& pieces,
                                           int tile, int row0, int rows, int warp, volatile int* flag,
-                                          Sync&& sync, Store&& store) {
+                                          float* weights, Sync&& sync, Store&& store) {
   const int lane = threadIdx.x & 31;
   auto arrive = [&](int first, int level, int n) {  // true in the last CTA to arrive
     sync();  // the others' rows before this thread's fence
@@ -336,29 +339,29 @@ __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPiec
     sync();
     return *flag != 0;
   };
-  auto finish = [&](int row, float4 o, float, float l) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    store(row, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-  };
-  const int n = pieces.count;
-  if (n <= kAttnFan) {
-    if (arrive(0, 0, n))
-      attn_merge<kWarps, R>(ws, pieces.list, 1, n, row0, rows, warp, finish);
+  auto whole = [](int, float, float l) { return l == 0.f ? 0.f : 1.f / l; };
+  int n = pieces.count, step = 1, first = 0;
+  if (n > kAttnFan) {
+    first = pieces.mine / kAttnFan * kAttnFan;
+    const int some = min(kAttnFan, n - first);
+    if (!arrive(first, 0, some)) return;
+    const int head = pieces.list[first];  // the group's result replaces its first piece
+    attn_merge<kWarps, R, U>(
+        ws, pieces.list + first, 1, some, row0, rows, warp, weights, sync,
+        [&](int row, float M, float l) {
+          reinterpret_cast<float2*>(ws.stats(head))[row] = make_float2(M, l);
+          return 1.f;
+        },
+        [&](int row, float4 o) {
+          reinterpret_cast<float4*>(ws.sums(head) + (long long)row * kHeadDim)[lane] = o;
+        });
+    n = (n + kAttnFan - 1) / kAttnFan;
+    step = kAttnFan;
+    if (!arrive(0, 1, n)) return;
+  } else if (!arrive(0, 0, n)) {
     return;
   }
-  const int first = pieces.mine / kAttnFan * kAttnFan, some = min(kAttnFan, n - first);
-  if (!arrive(first, 0, some)) return;
-  const int head = pieces.list[first];  // the group's result replaces its first piece
-  attn_merge<kWarps, R>(ws, pieces.list + first, 1, some, row0, rows, warp,
-                        [&](int row, float4 o, float M, float l) {
-                          reinterpret_cast<float4*>(ws.sums(head) + (long long)row * kHeadDim)[lane] = o;
-                          __syncwarp();
-                          if (lane == 0)
-                            reinterpret_cast<float2*>(ws.stats(head))[row] = make_float2(M, l);
-                        });
-  const int groups = (n + kAttnFan - 1) / kAttnFan;
-  if (arrive(0, 1, groups))
-    attn_merge<kWarps, R>(ws, pieces.list, kAttnFan, groups, row0, rows, warp, finish);
+  attn_merge<kWarps, R, U>(ws, pieces.list, step, n, row0, rows, warp, weights, sync, whole, store);
 }
 
 }  // namespace gdn

@@ -8,7 +8,7 @@
 //
 // Warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, scores read from TMEM and
 // P written back over them as the bf16 A operand of the second product.  Warp 8: issues the
-// products.  Warp 9: loads K and V tiles by TMA into a ring of five (K and V in turn), Q once
+// products.  Warp 9: loads K and V tiles by TMA into a ring of four (K and V in turn), Q once
 // per item.  (Warps 10 and 11 fill the register group.)  TMEM: S0 S1 O0 O1, 128 columns each.
 //
 // The maximum that a row's sums are relative to is raised only when the new one exceeds it
@@ -30,7 +30,7 @@ using namespace sm100;
 constexpr int kRows = 128;             // rows of a tile
 constexpr int kTile = kAttnTile;       // keys of a tile
 constexpr int kPart = 64;              // keys that a row's scores are taken for at once
-constexpr int kStages = 5;             // K / V ring
+constexpr int kStages = 4;             // K / V ring
 constexpr int kHalfBytes = 128 * 128;  // 64 columns of 128 rows, 128-byte swizzle
 constexpr int kTileBytes = 2 * kHalfBytes;
 constexpr int kThreads = 384;          // 168 registers a thread at launch: 64512
@@ -69,7 +69,8 @@ struct Shared {
   int failed, joining[2];
   float2 twin[kRows];  // (maximum, sum) of the second half's rows
 };
-constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + kStages * kTileBytes;
+constexpr int kStageOut = 4096;         // a softmax warp's buffer on the way out
+constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + kStages * kTileBytes + 8 * kStageOut;
 
 struct TcArgs {
   AttnArgs a;
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Shared sh;
   uint8_t* tiles = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   const uint32_t sq = smem_u32(tiles);
-  const uint32_t skv = sq + 2 * kTileBytes;
+  const uint32_t skv = sq + 2 * kTileBytes, sout = skv + kStages * kTileBytes;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const AttnArgs& a = p.a;
   const AttnGrid& g = p.g;
@@ -654,40 +655,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; ++i) o[i] = f0 * o[i] + f1 * o1[i];
           }
         };
+        // Out through the warp's buffer, 128 bytes of its 32 rows at a time: a row a thread, then
+        // a row to eight lanes (a store of 32 rows takes 32 turns, one of 4 rows 4).
+        const uint32_t buf = sout + warp * kStageOut;
+        const int wr = (warp & 3) * 32;  // the warp's first row
         if (slot < 0) {
           const float inv = 1.f / l;
-          __nv_bfloat16* op = a.out + (w.row0 + rtok) * a.o_stride +
-                              ((long long)w.head * grp + r % grp) * kHeadDim;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float o[32];
-            load(c, o);
-            if (mine) {
+          for (int c = 0; c < 2; ++c) {  // 64 columns of bf16
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+              float o[32];
+              load(2 * c + d, o);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 uint32_t pk[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                   pk[k] = saw ? pack_bf16(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv) : 0u;
-                *reinterpret_cast<uint4*>(op + 32 * c + 8 * i) =
-                    make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                st_shared_v4(buf + sw128(lane, 4 * d + i), pk[0], pk[1], pk[2], pk[3]);
               }
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int x = 4 * i + (lane >> 3), row = wr + x, tok = rt * g.sub + row / grp;
+              const uint4 v = ld_shared_v4(buf + sw128(x, lane & 7));
+              if (row < g.sub * grp && tok < w.toks)
+                *reinterpret_cast<uint4*>(a.out + (w.row0 + tok) * a.o_stride +
+                                          ((long long)w.head * grp + row % grp) * kHeadDim +
+                                          64 * c + 8 * (lane & 7)) = v;
+            }
+            __syncwarp();
           }
         } else {
           // a row that saw nothing of the piece: (-inf, 0), its sums are not read
           const int piece = 2 * blockIdx.x + slot;
-          float* po = p.ws.sums(piece) + (t * kRows + r) * kHeadDim;
+          float* po = p.ws.sums(piece) + (t * kRows + wr) * kHeadDim;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 4; ++c) {  // 32 columns of fp32
             float o[32];
             load(c, o);
-            if (saw) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float4*>(po + 32 * c + 4 * i) =
-                    make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            for (int i = 0; i < 8; ++i)
+              st_shared_v4(buf + sw128(lane, i), __float_as_uint(o[4 * i]),
+                           __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]),
+                           __float_as_uint(o[4 * i + 3]));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int x = 4 * i + (lane >> 3);
+              *reinterpret_cast<uint4*>(po + x * kHeadDim + 32 * c + 4 * (lane & 7)) =
+                  ld_shared_v4(buf + sw128(x, lane & 7));
             }
+            __syncwarp();
           }
           reinterpret_cast<float2*>(p.ws.stats(piece))[t * kRows + r] =
               saw ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
@@ -700,8 +721,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int toks = min(w.toks - t * g.sub, g.sub);
         if (slot >= 0 && toks > 0) {
           const long long out0 = w.row0 + t * g.sub;
-          attn_join<4, 8>(
+          attn_join<4, 8, 2>(
               p.ws, w.pieces, t, t * kRows, toks * grp, warp & 3, &sh.joining[t],
+              reinterpret_cast<float*>(tiles + (sout - sq) + 4 * t * kStageOut),
               [&] { group_sync(1 + t, 128); },
               [&](int row, float4 x) {
                 const int i = row - t * kRows;
@@ -750,7 +772,7 @@ cudaError_t launch_attn_tc(const AttnArgs& a, int sms, void* workspace, unsigned
   p.a = a;
   p.g.sub = kRows / grp;
   p.g.block = 2 * p.g.sub;
-  p.g.overhead = 128;
+  p.g.overhead = 384;
   p.g.whole = 4;
   p.ws = attn_partials(workspace, 2 * kRows, tag);
   CUtensorMap mq, mk, mv;
