@@ -87,14 +87,19 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
 
 }  // namespace
 
-bool attn_map(CUtensorMap* m, const void* base, long long d0, long long d1, long long d2,
-              long long s1, long long s2, int b1, int b2) {
+bool attn_map(CUtensorMap* m, const void* base, int rank, const long long* dims,
+              const long long* strides, const int* box) {
   auto fn = encoder();
-  if (!fn) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
-  const cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2}, one[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+  if (!fn || rank > 5) return false;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], one[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    b[i] = (cuuint32_t)box[i];
+    one[i] = 1;
+    if (i > 0) st[i - 1] = (cuuint64_t)strides[i - 1] * 2;
+  }
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, b,
             one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -107,11 +112,16 @@ int attn_key_box(const AttnArgs& p, int most) {
 
 bool attn_key_maps(CUtensorMap* mk, CUtensorMap* mv, const AttnArgs& p, int box) {
   const long long w = (long long)p.hkv * kHeadDim;
-  if (p.paged)
-    return attn_map(mk, p.k, w, p.page_size, p.num_pages, w, p.k_page_stride, box, 1) &&
-           attn_map(mv, p.v, w, p.page_size, p.num_pages, w, p.v_page_stride, box, 1);
-  return attn_map(mk, p.k, w, p.total_q, 1, p.k_stride, p.total_q * p.k_stride, box, 1) &&
-         attn_map(mv, p.v, w, p.total_q, 1, p.v_stride, p.total_q * p.v_stride, box, 1);
+  if (p.paged) {
+    // 64 columns, 8 rows, halves of the heads, groups of 8 rows of a page, pages
+    const long long dims[5] = {64, 8, 2 * p.hkv, p.page_size / 8, p.num_pages};
+    const long long ks[4] = {w, 64, 8 * w, p.k_page_stride}, vs[4] = {w, 64, 8 * w, p.v_page_stride};
+    const int b[5] = {64, 8, 2, box / 8, 1};
+    return attn_map(mk, p.k, 5, dims, ks, b) && attn_map(mv, p.v, 5, dims, vs, b);
+  }
+  const long long dims[2] = {w, p.total_q};
+  const int b[2] = {64, box};
+  return attn_map(mk, p.k, 2, dims, &p.k_stride, b) && attn_map(mv, p.v, 2, dims, &p.v_stride, b);
 }
 
 unsigned read_attn_device_error(bool clear) {

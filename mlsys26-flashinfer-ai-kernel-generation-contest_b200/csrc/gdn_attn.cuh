@@ -66,10 +66,12 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& p, int s) {
   return r;
 }
 
-// TMA maps: [d2][d1][d0] bf16, strides in elements, boxes of 64 x b1 x b2 with the 128-byte
-// swizzle; the maps of K and V (key rows of a page, or of the packed prompts), `box` rows high.
-bool attn_map(CUtensorMap* m, const void* base, long long d0, long long d1, long long d2,
-              long long s1, long long s2, int b1, int b2);
+// TMA map of a bf16 tensor (strides of dimensions 1 .. in elements), 128-byte swizzle; the
+// maps of K and V, `box` key rows high: rows of the packed prompts by halves of 64 columns, or
+// of a page, both halves for 8 rows after 8 rows (a head's 256 bytes of a row are asked for
+// together).
+bool attn_map(CUtensorMap* m, const void* base, int rank, const long long* dims,
+              const long long* strides, const int* box);
 bool attn_key_maps(CUtensorMap* mk, CUtensorMap* mv, const AttnArgs& p, int box);
 // The highest box (a power of two, at most `most`) that does not cross a page's end.
 int attn_key_box(const AttnArgs& p, int most);

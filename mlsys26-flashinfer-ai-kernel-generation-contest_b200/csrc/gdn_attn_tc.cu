@@ -236,6 +236,18 @@ __device__ __forceinline__ float exponentials(const float (&s)[2][32], float sca
   return v.x + v.y;
 }
 
+// Where a K or V tile's 128 keys lie in a stage (8-row groups of 64 columns, 1024 bytes each):
+// packed prompts one half of the columns after the other, pages both halves of a group.
+template <bool kPaged>
+struct TileLayout {
+  static constexpr uint32_t kHalf = kPaged ? 1024 : kHalfBytes;  // to the other 64 columns
+  static constexpr uint32_t kGroup = kPaged ? 2048 : 1024;       // to the next 8 keys
+  __device__ static __forceinline__ uint32_t row(uint32_t r) {
+    return (r >> 3) * kGroup + (r & 7) * 128;
+  }
+};
+
+template <bool kPaged>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv, const TcArgs p) {
@@ -248,6 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const AttnArgs& a = p.a;
   const AttnGrid& g = p.g;
   const int grp = a.hq / a.hkv;
+  using Layout = TileLayout<kPaged>;
 
   if (tid == 0) {
     Bars& b = sh.bars;
@@ -342,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         ++items;
-        const int* table = a.paged ? a.block_table + w.seq * a.table_stride : nullptr;
+        const int* table = kPaged ? a.block_table + w.seq * a.table_stride : nullptr;
         const int x = w.head * kHeadDim;
         for (int j = w.t0; j < w.t1 && ok; ++j) {
           for (int kv = 0; kv < 2; ++kv) {
@@ -357,20 +370,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             const uint32_t dst = skv + st * kTileBytes;
             const CUtensorMap* m = kv ? &mv : &mk;
-            for (int i = lane; i < kTile / p.box; i += 32) {
-              const int key = j * kTile + i * p.box;
-              int row, page;
-              if (table == nullptr) {
-                row = w.kv0 + key;
-                page = 0;
-              } else {
-                row = key % a.page_size;
-                page = key < w.kv_len ? __ldg(table + key / a.page_size) : -1;  // -1: not used
-                if (page < 0 || page >= a.num_pages) page = -1;  // no such page: zeros
+            if constexpr (kPaged) {
+              for (int i = lane; i < kTile / p.box; i += 32) {
+                const int key = j * kTile + i * p.box;
+                int page = key < w.kv_len ? __ldg(table + key / a.page_size) : -1;  // -1: not used
+                if (page >= a.num_pages || page < 0) page = -1;  // no such page: zeros
+                tma_load_5d(dst + i * p.box * 256, m, &bars.kv_full[st], 0, 0, 2 * w.head,
+                            key % a.page_size / 8, page);
               }
-              for (int h = 0; h < 2; ++h)
-                tma_load_3d(dst + h * kHalfBytes + i * p.box * 128, m, &bars.kv_full[st],
-                            x + 64 * h, row, page);
+            } else if (lane < 2) {
+              tma_load_2d(tiles + (dst - sq) + lane * kHalfBytes, m, &bars.kv_full[st],
+                          x + 64 * lane, w.kv0 + j * kTile);
             }
             ++ring;
           }
@@ -397,8 +407,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t = warp == 8 ? 0 : 1;
       constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPart, false, false);
       constexpr uint32_t idesc_o = umma_idesc_bf16(128, 128, false, true);
-      const uint64_t qdesc = umma_desc_k(sq), kdesc = umma_desc_k(skv);
-      const uint64_t vdesc = umma_desc_mn(skv, kHalfBytes);
+      const uint64_t qdesc = umma_desc_k(sq), kdesc = umma_desc_sw128(skv, 16, Layout::kGroup);
+      const uint64_t vdesc = umma_desc_sw128(skv, Layout::kHalf, Layout::kGroup);
       constexpr uint32_t kStep = kTileBytes >> 4;  // of a descriptor, to the next tile
       const uint32_t td = __shfl_sync(0xffffffffu, tmem, 0) + 128 * t;
       uint32_t tile0 = 0;         // K / V tiles before this piece
@@ -423,25 +433,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && elect_one()) mbar_arrive(&bars.kv_empty[entry % kStages]);
       };
       auto scores = [&](uint64_t q, uint32_t entry, int h) {  // S_h = Q K^T, keys 64 h ..
-        const uint64_t k = kdesc + entry % kStages * kStep + h * (kPart * 128 >> 4);
+        const uint64_t k = kdesc + entry % kStages * kStep + h * (kPart / 8 * Layout::kGroup >> 4);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const uint32_t off = ((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4;
-            umma_bf16(td + kPart * h, q + off, k + off, idesc_s, i > 0);
+            umma_bf16(td + kPart * h, q + (((i >> 2) * kHalfBytes + (i & 3) * 32) >> 4),
+                      k + (((i >> 2) * Layout::kHalf + (i & 3) * 32) >> 4), idesc_s, i > 0);
           }
           umma_commit(&bars.s_full[t][h]);
         }
       };
       auto values = [&](uint32_t entry, int h, bool first) {  // O += P_h V, keys 64 h ..
-        const uint64_t v = vdesc + entry % kStages * kStep + h * (kPart * 128 >> 4);
+        const uint64_t v = vdesc + entry % kStages * kStep + h * (kPart / 8 * Layout::kGroup >> 4);
         wait(&bars.p_ready[t][h], np, kErrTensor);
         tc_fence_after();
         if (ok && elect_one()) {
 #pragma unroll
           for (int i = 0; i < kPart / 16; ++i)
-            umma_bf16_tmem_a(td + 256, td + kPart * h + 8 * i, v + i * (2048 >> 4), idesc_o,
+            umma_bf16_tmem_a(td + 256, td + kPart * h + 8 * i, v + i * (2 * Layout::kGroup >> 4),
+                             idesc_o,
                              !first || i > 0);
           umma_commit(&bars.pv_done[t]);
         }
@@ -550,11 +561,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = __all_sync(0xffffffffu,
                           mbar_wait(&bars.kv_full[entry % kStages], entry / kStages & 1));
           if (ok && j * kTile + r >= kv_len) {
-            const uint32_t row = skv + entry % kStages * kTileBytes + r * 128;
+            const uint32_t row = skv + entry % kStages * kTileBytes + Layout::row(r);
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
               st_shared_v4(row + 16 * c, 0, 0, 0, 0);
-              st_shared_v4(row + kHalfBytes + 16 * c, 0, 0, 0, 0);
+              st_shared_v4(row + Layout::kHalf + 16 * c, 0, 0, 0, 0);
             }
           }
           fence_proxy_async();
@@ -776,21 +787,23 @@ cudaError_t launch_attn_tc(const AttnArgs& a, int sms, void* workspace, unsigned
   p.g.whole = 4;
   p.ws = attn_partials(workspace, 2 * kRows, tag);
   CUtensorMap mq, mk, mv;
-  bool ok = attn_map(&mq, a.q, kHeadDim, a.hq, a.total_q, kHeadDim, a.q_stride, grp, p.g.sub);
+  const long long qd[3] = {kHeadDim, a.hq, a.total_q}, qs[2] = {kHeadDim, a.q_stride};
+  const int qb[3] = {64, grp, p.g.sub};
+  bool ok = attn_map(&mq, a.q, 3, qd, qs, qb);
   p.box = attn_key_box(a, kTile);
   ok = ok && attn_key_maps(&mk, &mv, a, p.box);
   if (!ok) return cudaErrorInvalidValue;
-  static thread_local int set_for = -1;  // the attribute belongs to the device's context
+  auto* kernel = a.paged ? attn_tc_kernel<true> : attn_tc_kernel<false>;
+  static thread_local int set_for[2] = {-1, -1};  // the attribute belongs to the device's context
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (set_for != dev) {
-    e = cudaFuncSetAttribute(attn_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)kSmemBytes);
+  if (set_for[a.paged] != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e != cudaSuccess) return e;
-    set_for = dev;
+    set_for[a.paged] = dev;
   }
-  attn_tc_kernel<<<sms, kThreads, kSmemBytes, st>>>(mq, mk, mv, p);
+  kernel<<<sms, kThreads, kSmemBytes, st>>>(mq, mk, mv, p);
   return cudaGetLastError();
 }
 
