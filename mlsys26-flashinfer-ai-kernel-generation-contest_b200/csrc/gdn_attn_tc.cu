@@ -357,7 +357,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++items;
         const int* table = kPaged ? a.block_table + w.seq * a.table_stride : nullptr;
         const int x = w.head * kHeadDim;
+        // lane i: the page of the tile's box i, asked for a tile ahead
+        const int kv_len = w.kv_len, boxes = kTile / p.box;
+        auto page_of = [&](int j) {
+          const int key = j * kTile + lane * p.box;
+          if (!kPaged || lane >= boxes || key >= kv_len) return -1;  // -1: not used
+          return __ldg(table + key / a.page_size);
+        };
+        int page = page_of(w.t0);
         for (int j = w.t0; j < w.t1 && ok; ++j) {
+          const int next = j + 1 < w.t1 ? page_of(j + 1) : -1;
           for (int kv = 0; kv < 2; ++kv) {
             const uint32_t st = ring % kStages;
             if (ring >= kStages) ok = mbar_wait(&bars.kv_empty[st], (ring / kStages - 1) & 1);
@@ -371,12 +380,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t dst = skv + st * kTileBytes;
             const CUtensorMap* m = kv ? &mv : &mk;
             if constexpr (kPaged) {
-              for (int i = lane; i < kTile / p.box; i += 32) {
-                const int key = j * kTile + i * p.box;
-                int page = key < w.kv_len ? __ldg(table + key / a.page_size) : -1;  // -1: not used
-                if (page >= a.num_pages || page < 0) page = -1;  // no such page: zeros
-                tma_load_5d(dst + i * p.box * 256, m, &bars.kv_full[st], 0, 0, 2 * w.head,
-                            key % a.page_size / 8, page);
+              if (lane < boxes) {
+                const int key = j * kTile + lane * p.box;
+                tma_load_5d(dst + lane * p.box * 256, m, &bars.kv_full[st], 0, 0, 2 * w.head,
+                            key % a.page_size / 8,
+                            (unsigned)page < (unsigned)a.num_pages ? page : -1);  // none: zeros
               }
             } else if (lane < 2) {
               tma_load_2d(tiles + (dst - sq) + lane * kHalfBytes, m, &bars.kv_full[st],
@@ -384,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ++ring;
           }
+          page = next;
         }
         if (!ok) break;
         __syncwarp();
