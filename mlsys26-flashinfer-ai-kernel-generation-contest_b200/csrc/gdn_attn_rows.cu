@@ -35,7 +35,7 @@ constexpr int kRound = 16 * kWarps;  // keys that all groups take together
 constexpr int kWorks = 4;   // pieces handed out ahead
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr size_t smem_bytes(int rows) {  // ring, queries (later the join's weights)
-  static_assert(kAttnFan * sizeof(float) <= kHeadDim * 2, "the weights take the queries' place");
+  static_assert(attn_weight_bytes(1) <= kHeadDim * 2, "the weights take the queries' place");
   return 1024 + (size_t)kRing * kRound * 2 * kHeadDim * 2 + (size_t)rows * kHeadDim * 2;
 }
 
@@ -487,11 +487,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int head0 = w.head * grp;
         attn_join<kWarps, 1, 8>(
             p.ws, w.pieces, 0, 0, w.toks * grp, warp, &joining,
-            reinterpret_cast<float*>(raw + (sq - smem_u32(raw))),  // the queries are done with
+            raw + (sq - smem_u32(raw)),  // the queries are done with
             [] { group_sync(1, kWarps * 32); },
-            [&](int row, float4 x) {
-              *reinterpret_cast<uint2*>(a.out + (w.row0 + row / grp) * a.o_stride +
-                                        ((long long)head0 + row % grp) * kHeadDim + 4 * lane) =
+            [&](int row) {
+              return (w.row0 + row / grp) * a.o_stride +
+                     ((long long)head0 + row % grp) * kHeadDim;
+            },
+            [&](long long at, float4 x) {
+              *reinterpret_cast<uint2*>(a.out + at + 4 * lane) =
                   make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
             });
       }

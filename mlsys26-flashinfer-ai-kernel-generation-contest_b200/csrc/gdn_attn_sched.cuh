@@ -254,14 +254,20 @@ __device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& l
 
 // Joins `count` <= kAttnFan pieces list[0], list[step], .. of the rows [row0, row0 + rows),
 // by kWarps warps together (rows <= 32 kWarps).  First a thread takes a row's statistics and
-// leaves the pieces' weights in `weights` (kAttnFan x rows floats of shared memory), then a
-// warp takes R rows and U pieces at a time, all their loads in flight.  stat(row, maximum,
-// sum) gives what the row's weights are multiplied with, out(row, lane's four columns) gets
-// the weighted sums.
-template <int kWarps, int R, int U, typename Sync, typename Stat, typename Out>
+// leaves the pieces' weights in `weights` (shared memory, attn_weight_bytes(rows)) with the
+// row's place, then a warp takes R rows and U pieces at a time, all their loads in flight.
+// stat(row, maximum, sum) gives what the row's weights are multiplied with, place(row) where
+// it goes, out(place, lane's four columns) gets the weighted sums.
+__host__ __device__ constexpr int attn_weight_bytes(int rows) {
+  return rows * (kAttnFan * (int)sizeof(float) + (int)sizeof(long long));
+}
+template <int kWarps, int R, int U, typename Sync, typename Stat, typename Place, typename Out>
 __device__ __forceinline__ void attn_merge(const AttnPartials& ws, const short* list, int step,
                                            int count, int row0, int rows, int warp,
-                                           float* weights, Sync&& sync, Stat&& stat, Out&& out) {
+                                           void* weights_smem, Sync&& sync, Stat&& stat, Place&& place,
+                                           Out&& out) {
+  long long* places = static_cast<long long*>(weights_smem);
+  float* weights = reinterpret_cast<float*>(places + rows);
   const int lane = threadIdx.x & 31, r = warp * 32 + lane;
   if (r < rows) {
     float2 ml[kAttnFan];
@@ -280,6 +286,7 @@ __device__ __forceinline__ void attn_merge(const AttnPartials& ws, const short* 
       l += ml[i].y == 0.f ? 0.f : ml[i].x * ml[i].y;
     }
     const float f = stat(row0 + r, M, l);
+    places[r] = place(row0 + r);
 #pragma unroll
     for (int i = 0; i < kAttnFan; ++i)
       if (i < count) weights[i * rows + r] = ml[i].y == 0.f ? 0.f : ml[i].x * f;
@@ -316,18 +323,18 @@ __device__ __forceinline__ void attn_merge(const AttnPartials& ws, const short* 
     }
 #pragma unroll
     for (int j = 0; j < R; ++j)
-      if (r0 + j < rows) out(row0 + r0 + j, o[j]);
+      if (r0 + j < rows) out(places[r0 + j], o[j]);
   }
 }
 
 // After a piece's partial result is written: by the kWarps warps that wrote the rows [row0,
 // row0 + rows) (row tile `tile`) together, `sync` their barrier, `flag` an int of theirs in
-// shared memory, `weights` kAttnFan x rows floats.  The last CTA of an item to come here
-// writes its output through store(row, four columns).
-template <int kWarps, int R, int U, typename Sync, typename Store>
+// shared memory, `weights` attn_weight_bytes(rows) of theirs, 8-byte aligned.  The last CTA of
+// an item to come here writes its output through store(place(row), four columns).
+template <int kWarps, int R, int U, typename Sync, typename Place, typename Store>
 __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPieces& pieces,
                                           int tile, int row0, int rows, int warp, volatile int* flag,
-                                          float* weights, Sync&& sync, Store&& store) {
+                                          void* weights, Sync&& sync, Place&& place, Store&& store) {
   const int lane = threadIdx.x & 31;
   auto arrive = [&](int first, int level, int n) {  // true in the last CTA to arrive
     sync();  // the others' rows before this thread's fence
@@ -352,8 +359,9 @@ __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPiec
           reinterpret_cast<float2*>(ws.stats(head))[row] = make_float2(M, l);
           return 1.f;
         },
-        [&](int row, float4 o) {
-          reinterpret_cast<float4*>(ws.sums(head) + (long long)row * kHeadDim)[lane] = o;
+        [&](int row) { return (long long)row * kHeadDim; },
+        [&](long long at, float4 o) {
+          *reinterpret_cast<float4*>(ws.sums(head) + at + 4 * lane) = o;
         });
     n = (n + kAttnFan - 1) / kAttnFan;
     step = kAttnFan;
@@ -361,7 +369,8 @@ __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPiec
   } else if (!arrive(0, 0, n)) {
     return;
   }
-  attn_merge<kWarps, R, U>(ws, pieces.list, step, n, row0, rows, warp, weights, sync, whole, store);
+  attn_merge<kWarps, R, U>(ws, pieces.list, step, n, row0, rows, warp, weights, sync, whole, place,
+                           store);
 }
 
 }  // namespace gdn

@@ -70,6 +70,7 @@ struct Shared {
   float2 twin[kRows];  // (maximum, sum) of the second half's rows
 };
 constexpr int kStageOut = 4096;         // a softmax warp's buffer on the way out
+static_assert(attn_weight_bytes(kRows) <= 4 * kStageOut, "the join uses the buffers");
 constexpr size_t kSmemBytes = 1024 + 2 * kTileBytes + kStages * kTileBytes + 8 * kStageOut;
 
 struct TcArgs {
@@ -678,9 +679,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Out through the warp's buffer, 128 bytes of its 32 rows at a time: a row a thread, then
         // a row to eight lanes (a store of 32 rows takes 32 turns, one of 4 rows 4).
         const uint32_t buf = sout + warp * kStageOut;
-        const int wr = (warp & 3) * 32;  // the warp's first row
-        if (slot < 0) {
+        const int wr = (warp & 3) * 32;                                // the warp's first row
+        const int rows = min(w.toks - rt * g.sub, g.sub) * grp - wr;  // that are there, if > 0
+        if (rows <= 0) {
+          // nothing of this warp's
+        } else if (slot < 0) {
           const float inv = 1.f / l;
+          const long long mine_at = (w.row0 + rtok) * a.o_stride +
+                                    ((long long)w.head * grp + r % grp) * kHeadDim;
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {  // 64 columns of bf16
 #pragma unroll
@@ -699,12 +705,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int x = 4 * i + (lane >> 3), row = wr + x, tok = rt * g.sub + row / grp;
+              const int x = 4 * i + (lane >> 3);
+              const long long at = __shfl_sync(0xffffffffu, mine_at, x);
               const uint4 v = ld_shared_v4(buf + sw128(x, lane & 7));
-              if (row < g.sub * grp && tok < w.toks)
-                *reinterpret_cast<uint4*>(a.out + (w.row0 + tok) * a.o_stride +
-                                          ((long long)w.head * grp + row % grp) * kHeadDim +
-                                          64 * c + 8 * (lane & 7)) = v;
+              if (x < rows)
+                *reinterpret_cast<uint4*>(a.out + at + 64 * c + 8 * (lane & 7)) = v;
             }
             __syncwarp();
           }
@@ -725,8 +730,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int x = 4 * i + (lane >> 3);
-              *reinterpret_cast<uint4*>(po + x * kHeadDim + 32 * c + 4 * (lane & 7)) =
-                  ld_shared_v4(buf + sw128(x, lane & 7));
+              const uint4 v = ld_shared_v4(buf + sw128(x, lane & 7));
+              if (x < rows)
+                *reinterpret_cast<uint4*>(po + x * kHeadDim + 32 * c + 4 * (lane & 7)) = v;
             }
             __syncwarp();
           }
@@ -743,13 +749,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const long long out0 = w.row0 + t * g.sub;
           attn_join<4, 8, 2>(
               p.ws, w.pieces, t, t * kRows, toks * grp, warp & 3, &sh.joining[t],
-              reinterpret_cast<float*>(tiles + (sout - sq) + 4 * t * kStageOut),
+              tiles + (sout - sq) + 4 * t * kStageOut,
               [&] { group_sync(1 + t, 128); },
-              [&](int row, float4 x) {
+              [&](int row) {
                 const int i = row - t * kRows;
-                *reinterpret_cast<uint2*>(a.out + (out0 + i / grp) * a.o_stride +
-                                          ((long long)w.head * grp + i % grp) * kHeadDim +
-                                          4 * lane) =
+                return (out0 + i / grp) * a.o_stride +
+                       ((long long)w.head * grp + i % grp) * kHeadDim;
+              },
+              [&](long long at, float4 x) {
+                *reinterpret_cast<uint2*>(a.out + at + 4 * lane) =
                     make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
               });
         }
