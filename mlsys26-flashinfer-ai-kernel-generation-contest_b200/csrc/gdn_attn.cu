@@ -39,7 +39,7 @@ int parts() {
 // Rows of an item for the few-rows kernel, or 0 where the tensor-core kernel runs.
 int few_rows(long long total_q, int num_seqs, int hq, int hkv) {
   const long long rows = (total_q + num_seqs - 1) / num_seqs * (hq / hkv);
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
 }
 
 size_t workspace_size(long long total_q, int num_seqs, int hq, int hkv) {

@@ -28,15 +28,11 @@ namespace {
 
 using namespace sm100;
 
-constexpr int kWarps = 12;   // consumers
-constexpr int kRing = 2;     // chunks per group
 constexpr int kTile = kAttnTile;
-constexpr int kRound = 16 * kWarps;  // keys that all groups take together
 constexpr int kWorks = 4;   // pieces handed out ahead
-constexpr int kThreads = (kWarps + 1) * 32;
-constexpr size_t smem_bytes(int rows) {  // ring, queries (later the join's weights)
+constexpr size_t smem_bytes(int warps, int ring, int rows) {  // ring, queries (later the join's weights)
   static_assert(attn_weight_bytes(1) <= kHeadDim * 2, "the weights take the queries' place");
-  return 1024 + (size_t)kRing * kRound * 2 * kHeadDim * 2 + (size_t)rows * kHeadDim * 2;
+  return 1024 + (size_t)ring * 16 * warps * 2 * kHeadDim * 2 + (size_t)rows * kHeadDim * 2;
 }
 
 __device__ unsigned int g_rows_error = 0;
@@ -84,10 +80,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-template <int W, int NT>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int W, int NT, int kWarps, int kRing>
+__global__ void __launch_bounds__((kWarps + 1) * 32, 1)
     attn_rows_kernel(const __grid_constant__ RowsArgs p) {
   constexpr int kGroups = kWarps / W;
+  constexpr int kRound = 16 * kWarps;          // keys that all groups take together
   constexpr int kChunk = 16 * W;               // keys
   constexpr int kHalf = kChunk * 128;          // 64 columns of a chunk's K or V
   constexpr int kStage = 4 * kHalf;            // K, V
@@ -193,6 +190,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const long long page_stride = !a.paged ? 0 : lane < 16 ? a.k_page_stride : a.v_page_stride;
     const long long row_stride = a.paged ? (long long)a.hkv * kHeadDim
                                          : (lane < 16 ? a.k_stride : a.v_stride);
+    const bool runs = !a.paged || a.page_size % 16 == 0;  // a warp's 16 keys are in one page
+    uint32_t at_sw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      at_sw[i] = (uint32_t)((lane & 7) ^ ((2 * i + (lane >> 4)) & 7)) << 4;
     const int step_pages = a.paged ? kRound / a.page_size : 0;
     const int step_rows = kRound - step_pages * (a.paged ? a.page_size : 0);
     auto find_page = [&] {  // asked for a chunk ahead of its use
@@ -231,23 +233,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       const unsigned long long from = reinterpret_cast<unsigned long long>(
           there ? lbase + page * page_stride + lrow * row_stride : a.k);
       const uint32_t valid = __ballot_sync(0xffffffffu, there);
-      const uint32_t dst = stages + issued % kRing * kStage;
-      const int c = lane & 15;  // 16 bytes of a row
+      // lane: 16 bytes of a row, two rows at a time; `at_sw`: their swizzled places
+      const int c = lane & 15, hi = lane >> 4;
+      const uint32_t dst = stages + issued % kRing * kStage + (c >> 3) * kHalf + (mkey + hi) * 128;
+      if (runs && valid == 0xffffffffu) {  // 16 rows one after the other
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
+        for (int kv = 0; kv < 2; ++kv) {
+          const long long step = __shfl_sync(0xffffffffu, row_stride, 16 * kv) * 2;
+          unsigned long long at = __shfl_sync(0xffffffffu, from, 16 * kv) + hi * step + 16 * c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int k = 2 * i + (lane >> 4), src = 16 * kv + k;
-          const unsigned long long at = __shfl_sync(0xffffffffu, from, src) + 16 * c;
-          const uint32_t to = dst + (2 * kv + (c >> 3)) * kHalf + sw128(mkey + k, c & 7);
-          if (valid == 0xffffffffu)
-            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(to), "l"(at)
+          for (int i = 0; i < 8; ++i) {
+            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(
+                             dst + 2 * kv * kHalf + 256 * i + at_sw[i & 3]),
+                         "l"(at)
                          : "memory");
-          else
-            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(to),
+            at += 2 * step;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int src = 16 * kv + 2 * i + hi;
+            const unsigned long long at = __shfl_sync(0xffffffffu, from, src) + 16 * c;
+            asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(
+                             dst + 2 * kv * kHalf + 256 * i + at_sw[i & 3]),
                          "l"(at), "r"((valid >> src & 1) ? 16 : 0)
                          : "memory");
-        }
+          }
+      }
       asm volatile("cp.async.commit_group;" ::: "memory");
       ++issued;
       lkey += kRound;
@@ -314,8 +329,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t begun = done;
       for (int key0 = first; key0 < w.k1; key0 += kRound) {
         while (issued < done + kRing - 1 && open(n)) issue();
-        static_assert(kRing == 2, "one chunk is on its way");
-        asm volatile("cp.async.wait_group 0;" ::: "memory");  // this chunk has arrived
+        // this chunk has arrived: of the loads issued, all but the chunks behind it
+        if (kRing == 3 && issued > done + 1)
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+        static_assert(kRing == 2 || kRing == 3, "one or two chunks are on their way");
         if constexpr (W > 1) group_sync(2 + group, W * 32);
         else __syncwarp();
         if (open(n)) issue();  // into the stage of the chunk before, which everyone has left
@@ -509,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int W, int NT>
+template <int W, int NT, int kWarps, int kRing>
 cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long long tag,
                    cudaStream_t st) {
   const int grp = a.hq / a.hkv;
@@ -526,12 +545,13 @@ cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long lo
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (set_for != dev) {
-    e = cudaFuncSetAttribute(attn_rows_kernel<W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem_bytes(rows));
+    e = cudaFuncSetAttribute(attn_rows_kernel<W, NT, kWarps, kRing>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem_bytes(kWarps, kRing, rows));
     if (e != cudaSuccess) return e;
     set_for = dev;
   }
-  attn_rows_kernel<W, NT><<<sms, kThreads, smem_bytes(rows), st>>>(p);
+  attn_rows_kernel<W, NT, kWarps, kRing>
+      <<<sms, (kWarps + 1) * 32, smem_bytes(kWarps, kRing, rows), st>>>(p);
   return cudaGetLastError();
 }
 
@@ -549,10 +569,9 @@ unsigned read_attn_rows_error(bool clear) {
 
 cudaError_t launch_attn_rows(const AttnArgs& p, int rows, int sms, void* workspace,
                              unsigned long long tag, cudaStream_t st) {
-  return rows == 8    ? launch<1, 1>(p, sms, workspace, tag, st)
-         : rows == 16 ? launch<1, 2>(p, sms, workspace, tag, st)
-         : rows == 32 ? launch<2, 2>(p, sms, workspace, tag, st)
-                      : launch<4, 2>(p, sms, workspace, tag, st);
+  return rows == 8    ? launch<1, 1, 12, 2>(p, sms, workspace, tag, st)
+         : rows == 16 ? launch<2, 1, 12, 2>(p, sms, workspace, tag, st)
+                      : launch<4, 1, 12, 2>(p, sms, workspace, tag, st);
 }
 
 }  // namespace gdn
