@@ -504,7 +504,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
       }
       if (w.slot >= 0) {
         const int head0 = w.head * grp;
-        attn_join<kWarps, 1, 8>(
+        attn_join<kWarps, 1, 16>(
             p.ws, w.pieces, 0, 0, w.toks * grp, warp, &joining,
             raw + (sq - smem_u32(raw)),  // the queries are done with
             [] { group_sync(1, kWarps * 32); },
@@ -539,6 +539,7 @@ cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long lo
   p.g.block = p.g.sub;
   p.g.overhead = 128;
   p.g.whole = 8;
+  p.g.least = 768;
   p.ws = attn_partials(workspace, rows, tag);
   static thread_local int set_for = -1;  // the attribute belongs to the device's context
   int dev = 0;

@@ -26,6 +26,7 @@ struct AttnGrid {
   int sub;       // query tokens per tile of rows
   int overhead;  // cost of an item's start and end, in keys
   int whole;     // items of at most this many tiles are not split
+  int least;     // cost below which a CTA's share is not worth a split
 };
 
 // Quotients of costs: 32 bits where they do (a 64-bit division is some 100 instructions).
@@ -47,6 +48,7 @@ __device__ __forceinline__ int attn_blocks(const AttnSeq& s, int block) {
 __device__ __forceinline__ long long attn_cost_before(const AttnSeq& s, const AttnGrid& g, int n) {
   if (n <= 0) return 0;
   const int nb = attn_blocks(s, g.block);
+  if (nb == 1) return (long long)s.kv_len + g.overhead;  // as the rest would give
   const long long a = (long long)s.kv_len - s.q_len;
   const long long m = n < nb ? n : nb - 1;              // blocks of full size
   long long b0 = a < 0 ? (unsigned)-a / (unsigned)g.block : 0;              // leading blocks that see nothing
@@ -136,13 +138,27 @@ __device__ __forceinline__ AttnShare attn_share(const AttnArgs& p, const AttnGri
   const int lane = threadIdx.x & 31;
   AttnShare r;
   long long cost = 0, mine = 0;  // of the lane's last sequence, of all of them
+  int items = 0;
 #pragma unroll 4
   for (int s = lane; s < p.num_seqs; s += 32) {
-    cost = attn_head_cost(attn_seq(p, s), g) * p.hkv;
+    const AttnSeq seq = attn_seq(p, s);
+    cost = attn_head_cost(seq, g) * p.hkv;
     mine += cost;
+    items += min(attn_blocks(seq, g.block) * p.hkv, parts);
   }
 #pragma unroll
-  for (int w = 1; w < 32; w <<= 1) mine += __shfl_xor_sync(0xffffffffu, mine, w);
+  for (int w = 1; w < 32; w <<= 1) {
+    mine += __shfl_xor_sync(0xffffffffu, mine, w);
+    items += min(__shfl_xor_sync(0xffffffffu, items, w), parts);  // (only below `parts` counts)
+  }
+  // Little work is not cut into as many pieces as there are CTAs, whose join would cost more
+  // than it saves: shares of `least` at least, but four for each item, so that items that are
+  // not split find a CTA each.
+  if (4 * items < parts) {
+    const long long some = attn_div(mine, g.least);
+    parts = some < 4 * items ? 4 * items : some < parts ? (int)some : parts;
+    if (parts < 1) parts = 1;
+  }
   r.line.total = mine;
   r.line.per = attn_div(mine, parts);
   r.line.rest = (int)(mine - r.line.per * parts);
@@ -151,7 +167,8 @@ __device__ __forceinline__ AttnShare attn_share(const AttnArgs& p, const AttnGri
   r.u1 = r.line.cut(c + 1);
   r.seq = 0;
   r.seq_start = 0;
-  if (r.u0 >= r.u1) return r;  // no work: the line is shorter than the number of CTAs
+  if (c >= parts) r.u1 = r.u0;
+  if (r.u0 >= r.u1) return r;  // no work
   long long base = 0;
   for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
     if (p.num_seqs > 32) {

@@ -802,6 +802,7 @@ cudaError_t launch_attn_tc(const AttnArgs& a, int sms, void* workspace, unsigned
   p.g.block = 2 * p.g.sub;
   p.g.overhead = 384;
   p.g.whole = 4;
+  p.g.least = 1024;
   p.ws = attn_partials(workspace, 2 * kRows, tag);
   CUtensorMap mq, mk, mv;
   const long long qd[3] = {kHeadDim, a.hq, a.total_q}, qs[2] = {kHeadDim, a.q_stride};
