@@ -221,18 +221,22 @@ inline AttnPartials attn_partials(void* workspace, int rows, unsigned long long 
                       rows};
 }
 // A counter's memory may hold anything before the first arrival: only a word with this
-// launch's tag counts.  The last of n arrivals (true) clears it, for the next replay of a
-// captured launch, whose tag is the same.
+// launch's tag counts.  The first arrival puts it there; whoever finds that done just adds,
+// so that no arrival waits for others' (a loop of compare-and-swaps by 16 CTAs that finish
+// together took 8 us).  The last of n arrivals (true) clears the word, for the next replay
+// of a captured launch, whose tag is the same.
 __device__ __forceinline__ bool attn_arrive(unsigned long long* word, unsigned long long tag,
                                             int n) {
-  unsigned long long seen = *static_cast<volatile unsigned long long*>(word);
-  while (true) {
-    const unsigned long long k = ((seen >> 16) == tag ? (seen & 0xffffu) : 0u) + 1;
-    const bool last = k == (unsigned long long)n;
-    const unsigned long long was = atomicCAS(word, seen, last ? 0ull : (tag << 16) | k);
-    if (was == seen) return last;
+  const unsigned long long first = (tag << 16) | 1;
+  unsigned long long seen = 0, was = atomicCAS(word, seen, first);  // cleared by an earlier launch?
+  if (was != seen && (was >> 16) != tag) {
     seen = was;
+    was = atomicCAS(word, seen, first);
   }
+  int k = 1;
+  if (was != seen) k = (int)(atomicAdd(word, 1ull) & 0xffffu) + 1;  // it has the tag
+  if (k == n) atomicExch(word, 0ull);
+  return k == n;
 }
 
 // The pieces of one item, in the order of the keys, as every one of its CTAs finds them.

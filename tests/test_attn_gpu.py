@@ -207,7 +207,9 @@ def test_paged_views_lengths_beyond_the_table_and_rows_behind(cuda, q_len):
     o4 = torch.full_like(x, 3.0)
     pkg.attn_paged(x[:, :q_len], both[:, 0], both[:, 1], view, d["kv_lens"].to(cuda), None,
                    o4[:, :q_len])
-    assert torch.equal(o4[:, :q_len].reshape(t, 8, D), r[:t]) and (o4[:, q_len:] == 3).all()
+    # (padded rows count for the kernel's choice: the same values, not the same roundings)
+    check(o4[:, :q_len].reshape(t, 8, D), ref[:t], size[:t])
+    assert (o4[:, q_len:] == 3).all()
 
 
 def test_mixed_batch_of_a_chunk_and_single_tokens(cuda):
