@@ -29,10 +29,11 @@ struct RopeArgs {
   __nv_bfloat16 *k_cache, *v_cache;  // null: k_out is written instead
   long long q_stride, k_stride, v_stride, qo_stride, ko_stride;
   long long k_page_stride, v_page_stride, num_slots, table_rows;
-  long long groups;  // tokens * groups of heads
+  unsigned groups;  // tokens * groups of heads
   float eps;
   int hq, hkv, rd, page_size, groups_per_token;
-  bool pos64, slot64;
+  int batches;  // of HPG heads in a group
+  bool pos64, slot64, wide;  // wide: a lane's table values are whole 16-byte pieces
 };
 
 __device__ __forceinline__ long long load_index(const void* p, bool is64, long long i) {
@@ -49,31 +50,34 @@ __device__ __forceinline__ float sum16(float x) {
 
 enum RopeLayout { kInterleaved = 0, kHalfAligned = 1, kHalfAny = 2 };
 
-// One half-warp per group of HPG heads of one token: the table row is read once for them
-// and their loads are in flight together.
+// One half-warp per group of heads of one token, HPG at a time: the table row is read once
+// for the group, a batch's loads are in flight together, and with the batch before's work.
 template <int HPG, int LAYOUT>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeArgs p) {
+__global__ void __launch_bounds__(256, HPG > 1 ? 3 : 1) rope_kernel(const RopeArgs p) {
   __shared__ float stage[LAYOUT == kHalfAny ? 16 : 1][kHeadDim];
   const int lane = threadIdx.x & 15;
-  const long long group = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const unsigned group = blockIdx.x * 16 + (threadIdx.x >> 4);
   const bool live = group < p.groups;
   // lanes of a dead half-warp go along with the shuffles on group 0's values
-  const long long g = live ? group : 0;
-  const long long t = g / p.groups_per_token;
-  const int h0 = (int)(g - t * p.groups_per_token) * HPG;
+  const unsigned g = live ? group : 0, token = g / (unsigned)p.groups_per_token;
+  const long long t = token;
+  int h0 = (int)(g - token * p.groups_per_token) * p.batches * HPG;
   const int heads = p.hq + p.hkv + (p.k_cache != nullptr ? p.hkv : 0);
 
   uint4 raw[HPG];
+  auto load = [&](int from) {
 #pragma unroll
-  for (int i = 0; i < HPG; ++i) {
-    const int h = h0 + i;
-    const __nv_bfloat16* src =
-        h < p.hq ? p.q + t * p.q_stride + (long long)h * kHeadDim
-        : h < p.hq + p.hkv
-            ? p.k + t * p.k_stride + (long long)(h - p.hq) * kHeadDim
-            : p.v + t * p.v_stride + (long long)(h - p.hq - p.hkv) * kHeadDim;
-    raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + 8 * lane) : make_uint4(0, 0, 0, 0);
-  }
+    for (int i = 0; i < HPG; ++i) {
+      const int h = from + i;
+      const __nv_bfloat16* src =
+          h < p.hq ? p.q + t * p.q_stride + (long long)h * kHeadDim
+          : h < p.hq + p.hkv
+              ? p.k + t * p.k_stride + (long long)(h - p.hq) * kHeadDim
+              : p.v + t * p.v_stride + (long long)(h - p.hq - p.hkv) * kHeadDim;
+      raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + 8 * lane) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(h0);
 
   const long long pos = load_index(p.positions, p.pos64, t);
   const bool known = pos >= 0 && pos < p.table_rows;  // else: a padding token
@@ -82,98 +86,135 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeArgs p) {
     slot = load_index(p.slots, p.slot64, t);
     if (slot >= p.num_slots) slot = -1;
   }
-  const long long page = slot >= 0 ? slot / p.page_size : 0;
+  const long long page = slot < 0            ? 0
+                         : slot >> 32 == 0 ? (unsigned)slot / (unsigned)p.page_size
+                                           : slot / p.page_size;
   const long long off = slot >= 0 ? slot - page * p.page_size : 0;
 
   // cos / sin of the lane's 8 values (1, 0 where nothing turns)
   const int half = p.rd >> 1;
   float c[8], s[8];
   const float* row = p.table + (known ? pos : 0) * (long long)p.rd;  // not read unless known
+  if (p.wide) {  // the lane's 8 values turn, or none does
+    const bool turns = known && 8 * lane < p.rd;
+    if constexpr (LAYOUT == kInterleaved) {
+      const float4 one = make_float4(1.f, 1.f, 1.f, 1.f), none = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 x = turns ? __ldg(reinterpret_cast<const float4*>(row) + lane) : one;
+      const float4 y = turns ? __ldg(reinterpret_cast<const float4*>(row + half) + lane) : none;
+      c[0] = c[1] = x.x; c[2] = c[3] = x.y; c[4] = c[5] = x.z; c[6] = c[7] = x.w;
+      s[1] = y.x; s[3] = y.y; s[5] = y.z; s[7] = y.w;
+      s[0] = -y.x; s[2] = -y.y; s[4] = -y.z; s[6] = -y.w;
+    } else {
+      const bool front = 8 * lane < half;  // the first of a pair takes -s of the second
+      const int i = front ? 8 * lane : 8 * lane - half;
+      const float4 one = make_float4(1.f, 1.f, 1.f, 1.f), none = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4* pc = reinterpret_cast<const float4*>(row + (turns ? i : 0));
+      const float4* ps = reinterpret_cast<const float4*>(row + half + (turns ? i : 0));
+      const float4 x = turns ? __ldg(pc) : one, x2 = turns ? __ldg(pc + 1) : one;
+      const float4 y = turns ? __ldg(ps) : none, y2 = turns ? __ldg(ps + 1) : none;
+      const float sign = front ? -1.f : 1.f;
+      c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
+      c[4] = x2.x; c[5] = x2.y; c[6] = x2.z; c[7] = x2.w;
+      s[0] = sign * y.x; s[1] = sign * y.y; s[2] = sign * y.z; s[3] = sign * y.w;
+      s[4] = sign * y2.x; s[5] = sign * y2.y; s[6] = sign * y2.z; s[7] = sign * y2.w;
+    }
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int d = 8 * lane + e;
-    const int i = LAYOUT == kInterleaved ? d >> 1 : (d < half ? d : d - half);
-    const bool turns = known && d < p.rd;
-    c[e] = turns ? __ldg(row + i) : 1.f;
-    s[e] = turns ? __ldg(row + half + i) : 0.f;
-    // the first of a pair takes -s of the second
-    if (LAYOUT == kInterleaved ? (d & 1) == 0 : d < half) s[e] = -s[e];
+    for (int e = 0; e < 8; ++e) {
+      const int d = 8 * lane + e;
+      const int i = LAYOUT == kInterleaved ? d >> 1 : (d < half ? d : d - half);
+      const bool turns = known && d < p.rd;
+      c[e] = turns ? __ldg(row + i) : 1.f;
+      s[e] = turns ? __ldg(row + half + i) : 0.f;
+      // the first of a pair takes -s of the second
+      if (LAYOUT == kInterleaved ? (d & 1) == 0 : d < half) s[e] = -s[e];
+    }
   }
   // half layout: the lane that holds the partners
   const int step = half >> 3;
   const int partner = 8 * lane < half ? lane + step : (8 * lane < p.rd ? lane - step : lane);
 
+  for (int b = 0;; h0 += HPG) {
+    uint4 now[HPG];
 #pragma unroll
-  for (int i = 0; i < HPG; ++i) {
-    const int h = h0 + i;
-    const bool is_v = h >= p.hq + p.hkv;
-    float x[8];
-    {
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    for (int i = 0; i < HPG; ++i) now[i] = raw[i];
+    const bool last = ++b == p.batches;
+    if (!last) load(h0 + HPG);
+#pragma unroll
+    for (int i = 0; i < HPG; ++i) {
+      const int h = h0 + i;
+      const bool is_v = h >= p.hq + p.hkv;
+      float x[8];
+      {
+        const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = bf2x2_to_f2(w[e]);
+          x[2 * e] = f.x;
+          x[2 * e + 1] = f.y;
+        }
+      }
+      const float* weight = h < p.hq ? p.q_weight : p.k_weight;
+      if (p.q_weight != nullptr || p.k_weight != nullptr) {  // (all lanes take the shuffles)
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        ss = sum16(ss);
+        if (weight != nullptr && !is_v) {
+          const float r = rsqrtf(ss * (1.f / kHeadDim) + p.eps);
+          const float4 w0 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane);
+          const float4 w1 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane + 1);
+          x[0] *= r * w0.x; x[1] *= r * w0.y; x[2] *= r * w0.z; x[3] *= r * w0.w;
+          x[4] *= r * w1.x; x[5] *= r * w1.y; x[6] *= r * w1.z; x[7] *= r * w1.w;
+        }
+      }
+      float y[8];
+      if constexpr (LAYOUT == kInterleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
+      } else if constexpr (LAYOUT == kHalfAligned) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner, 16);
+      } else {
+        float* st = stage[threadIdx.x >> 4];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) st[8 * lane + e] = x[e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = 8 * lane + e;
+          y[e] = d < p.rd ? st[d < half ? d + half : d - half] : 0.f;
+        }
+      }
+      uint4 o;
+      uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 f = bf2x2_to_f2(w[e]);
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
+        const int d = 8 * lane + 2 * e;  // rd is even: both values turn or neither does
+        const float a = d < p.rd ? fmaf(x[2 * e], c[2 * e], y[2 * e] * s[2 * e]) : x[2 * e];
+        const float b = d < p.rd ? fmaf(x[2 * e + 1], c[2 * e + 1], y[2 * e + 1] * s[2 * e + 1])
+                                 : x[2 * e + 1];
+        const __nv_bfloat162 b2 = __floats2bfloat162_rn(a, b);
+        w[e] = *reinterpret_cast<const uint32_t*>(&b2);
       }
-    }
-    const float* weight = h < p.hq ? p.q_weight : p.k_weight;
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-    ss = sum16(ss);
-    if (weight != nullptr && !is_v) {
-      const float r = rsqrtf(ss * (1.f / kHeadDim) + p.eps);
-      const float4 w0 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane);
-      const float4 w1 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane + 1);
-      x[0] *= r * w0.x; x[1] *= r * w0.y; x[2] *= r * w0.z; x[3] *= r * w0.w;
-      x[4] *= r * w1.x; x[5] *= r * w1.y; x[6] *= r * w1.z; x[7] *= r * w1.w;
-    }
-    float y[8];
-    if constexpr (LAYOUT == kInterleaved) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
-    } else if constexpr (LAYOUT == kHalfAligned) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(0xffffffffu, x[e], partner, 16);
-    } else {
-      float* st = stage[threadIdx.x >> 4];
-      __syncwarp();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) st[8 * lane + e] = x[e];
-      __syncwarp();
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = 8 * lane + e;
-        y[e] = d < p.rd ? st[d < half ? d + half : d - half] : 0.f;
+      o = is_v ? now[i] : known ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0, 0, 0, 0);
+      if (!live || h >= heads) continue;
+      __nv_bfloat16* dst;
+      if (h < p.hq) {
+        dst = p.q_out + t * p.qo_stride + (long long)h * kHeadDim;
+      } else if (p.k_cache == nullptr) {
+        dst = p.k_out + t * p.ko_stride + (long long)(h - p.hq) * kHeadDim;
+      } else {
+        if (slot < 0) continue;
+        dst = is_v ? p.v_cache + page * p.v_page_stride +
+                         (off * p.hkv + (h - p.hq - p.hkv)) * (long long)kHeadDim
+                   : p.k_cache + page * p.k_page_stride +
+                         (off * p.hkv + (h - p.hq)) * (long long)kHeadDim;
       }
+      *reinterpret_cast<uint4*>(dst + 8 * lane) = o;
     }
-    uint4 o;
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int d = 8 * lane + 2 * e;  // rd is even: both values turn or neither does
-      const float a = d < p.rd ? fmaf(x[2 * e], c[2 * e], y[2 * e] * s[2 * e]) : x[2 * e];
-      const float b = d < p.rd ? fmaf(x[2 * e + 1], c[2 * e + 1], y[2 * e + 1] * s[2 * e + 1])
-                               : x[2 * e + 1];
-      const __nv_bfloat162 b2 = __floats2bfloat162_rn(a, b);
-      w[e] = *reinterpret_cast<const uint32_t*>(&b2);
-    }
-    o = is_v ? raw[i] : known ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0, 0, 0, 0);
-    if (!live || h >= heads) continue;
-    __nv_bfloat16* dst;
-    if (h < p.hq) {
-      dst = p.q_out + t * p.qo_stride + (long long)h * kHeadDim;
-    } else if (p.k_cache == nullptr) {
-      dst = p.k_out + t * p.ko_stride + (long long)(h - p.hq) * kHeadDim;
-    } else {
-      if (slot < 0) continue;
-      dst = is_v ? p.v_cache + page * p.v_page_stride +
-                       (off * p.hkv + (h - p.hq - p.hkv)) * (long long)kHeadDim
-                 : p.k_cache + page * p.k_page_stride +
-                       (off * p.hkv + (h - p.hq)) * (long long)kHeadDim;
-    }
-    *reinterpret_cast<uint4*>(dst + 8 * lane) = o;
+    if (last) break;
   }
 }
 
@@ -267,9 +308,17 @@ extern "C" int gdn_attn_qk_norm_rope_launch(
   const int layout =
       interleaved ? kInterleaved : (rotary_dim % 16 == 0 ? kHalfAligned : kHalfAny);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  constexpr int hpg = 4;
-  p.groups_per_token = (heads + hpg - 1) / hpg;
-  p.groups = (long long)num_tokens * p.groups_per_token;
-  if ((p.groups + 15) / 16 > 0x7fffffffLL) return GDN_ERR_INVALID_ARGUMENT;
-  return launch_rope<hpg>(p, layout, st) == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
+  p.wide = misaligned(rope_table, 16) == 0 &&
+           (interleaved ? rotary_dim % 8 == 0 : layout == kHalfAligned && rotary_dim % 16 == 0);
+  // A half-warp takes all heads of a token, four at a time, where there are tokens enough to
+  // fill the card (32768 tokens of 20 heads: 69.8 us, four heads a half-warp 88 us), four
+  // heads where not, and one where even that leaves SMs idle (7 tokens: 3.4 us, four 4.0 us).
+  const int hpg = (long long)num_tokens * heads <= 16 * 148 ? 1 : 4;
+  p.batches = num_tokens >= 4096 ? (heads + hpg - 1) / hpg : 1;
+  p.groups_per_token = (heads + hpg * p.batches - 1) / (hpg * p.batches);
+  const long long groups = (long long)num_tokens * p.groups_per_token;
+  if (groups > 0x7fffffffLL) return GDN_ERR_INVALID_ARGUMENT;
+  p.groups = (unsigned)groups;
+  const cudaError_t err = hpg == 1 ? launch_rope<1>(p, layout, st) : launch_rope<4>(p, layout, st);
+  return err == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }
