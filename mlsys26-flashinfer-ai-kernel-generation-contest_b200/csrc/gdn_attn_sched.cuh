@@ -81,17 +81,19 @@ struct AttnCursor {
     h = 0;
     b = 0;
   }
-  // To the item that holds cost u, in sequence s whose cost begins at `at`.
+  // To the item that holds cost u, in sequence s whose cost begins at `at` (by a whole warp).
   __device__ __forceinline__ void seek(const AttnArgs& p, const AttnGrid& g, int seq_index,
                                        long long at, long long u) {
     open(p, g, seq_index);
     const long long per = attn_head_cost(seq, g);
     h = (int)attn_div(u - at, per);
     const long long r = u - at - h * per;
-    int lo = 0, hi = nb - 1;  // the last block whose cost begins at or before r
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (attn_cost_before(seq, g, mid) <= r) lo = mid; else hi = mid - 1;
+    int lo = 0, hi = nb;  // the last block whose cost begins at or before r: in [lo, hi)
+    while (hi - lo > 1) {  // 32 places at a time
+      const int step = (hi - lo + 31) / 32, n = lo + (int)(threadIdx.x & 31) * step;
+      const bool before = n < hi && attn_cost_before(seq, g, n) <= r;
+      lo += (__popc(__ballot_sync(0xffffffffu, before)) - 1) * step;
+      hi = min(hi, lo + step);
     }
     b = lo;
     start = at + h * per + attn_cost_before(seq, g, b);

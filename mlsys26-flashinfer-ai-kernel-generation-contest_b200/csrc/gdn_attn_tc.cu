@@ -663,11 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const bool both = twin && t1 > t0 + 1;      // O_1 holds something
         const bool saw = mine && lim > t0 * kTile;  // some key of the piece
-        auto load = [&](int c, float(&o)[32]) {     // 32 columns of the row's sums
-          if (has) {
-            tmem_ld32(to + 32 * c, o);
-            tmem_wait_ld();
-          }
+        auto load = [&](int c, float(&o)[32]) {     // 32 columns of the row's sums, asked for
+          if (has) tmem_ld32(to + 32 * c, o);
+        };
+        auto with_twin = [&](int c, float(&o)[32]) {
           if (both) {
             float o1[32];
             tmem_ld32(to + 128 + 32 * c, o1);
@@ -687,18 +686,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float inv = 1.f / l;
           const long long mine_at = (w.row0 + rtok) * a.o_stride +
                                     ((long long)w.head * grp + r % grp) * kHeadDim;
+          __nv_bfloat16* at[8];  // where the lane's rows go
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            at[i] = a.out + __shfl_sync(0xffffffffu, mine_at, 4 * i + (lane >> 3)) + 8 * (lane & 7);
 #pragma unroll 1
           for (int c = 0; c < 2; ++c) {  // 64 columns of bf16
+            float o[2][32];
+            load(2 * c, o[0]);
+            load(2 * c + 1, o[1]);
+            tmem_wait_ld();
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
-              float o[32];
-              load(2 * c + d, o);
+              with_twin(2 * c + d, o[d]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 uint32_t pk[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  pk[k] = saw ? pack_bf16(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv) : 0u;
+                  pk[k] = saw ? pack_bf16(o[d][8 * i + 2 * k] * inv, o[d][8 * i + 2 * k + 1] * inv)
+                              : 0u;
                 st_shared_v4(buf + sw128(lane, 4 * d + i), pk[0], pk[1], pk[2], pk[3]);
               }
             }
@@ -706,10 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int x = 4 * i + (lane >> 3);
-              const long long at = __shfl_sync(0xffffffffu, mine_at, x);
               const uint4 v = ld_shared_v4(buf + sw128(x, lane & 7));
-              if (x < rows)
-                *reinterpret_cast<uint4*>(a.out + at + 64 * c + 8 * (lane & 7)) = v;
+              if (x < rows) *reinterpret_cast<uint4*>(at[i] + 64 * c) = v;
             }
             __syncwarp();
           }
@@ -721,6 +726,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 4; ++c) {  // 32 columns of fp32
             float o[32];
             load(c, o);
+            tmem_wait_ld();
+            with_twin(c, o);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               st_shared_v4(buf + sw128(lane, i), __float_as_uint(o[4 * i]),
