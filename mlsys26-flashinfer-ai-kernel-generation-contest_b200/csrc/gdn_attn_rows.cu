@@ -539,6 +539,7 @@ cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long lo
   p.g.block = p.g.sub;
   p.g.overhead = 128;
   p.g.whole = 8;
+  p.g.snap = 3;
   p.g.least = 768;
   p.ws = attn_partials(workspace, rows, tag);
   static thread_local int set_for = -1;  // the attribute belongs to the device's context

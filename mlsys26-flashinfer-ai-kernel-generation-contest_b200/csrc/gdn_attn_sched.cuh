@@ -26,6 +26,7 @@ struct AttnGrid {
   int sub;       // query tokens per tile of rows
   int overhead;  // cost of an item's start and end, in keys
   int whole;     // items of at most this many tiles are not split
+  int snap;      // a cut nearer to an item's end than this many tiles goes to the end
   int least;     // cost below which a CTA's share is not worth a split
 };
 
@@ -66,7 +67,8 @@ __device__ __forceinline__ int attn_tile_at(const AttnGrid& g, int e, int n, lon
   if (x >= cost) return n;
   if (n <= g.whole) return 2 * x > cost ? n : 0;
   const long long y = x - g.overhead;
-  return y <= 0 ? 0 : (int)((unsigned long long)y / kAttnTile);
+  const int t = y <= 0 ? 0 : (int)((unsigned long long)y / kAttnTile);
+  return t < g.snap ? 0 : n - t < g.snap ? n : t;
 }
 
 struct AttnCursor {

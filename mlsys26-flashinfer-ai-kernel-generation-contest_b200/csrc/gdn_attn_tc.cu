@@ -807,8 +807,9 @@ cudaError_t launch_attn_tc(const AttnArgs& a, int sms, void* workspace, unsigned
   p.a = a;
   p.g.sub = kRows / grp;
   p.g.block = 2 * p.g.sub;
-  p.g.overhead = 384;
+  p.g.overhead = 320;
   p.g.whole = 4;
+  p.g.snap = 3;
   p.g.least = 1024;
   p.ws = attn_partials(workspace, 2 * kRows, tag);
   CUtensorMap mq, mk, mv;
