@@ -148,12 +148,13 @@ __device__ __forceinline__ AttnShare attn_share(const AttnArgs& p, const AttnGri
     const AttnSeq seq = attn_seq(p, s);
     cost = attn_head_cost(seq, g) * p.hkv;
     mine += cost;
-    items += min(attn_blocks(seq, g.block) * p.hkv, parts);
+    items = min(items + (int)min((long long)attn_blocks(seq, g.block) * p.hkv, (long long)parts),
+                parts);  // (only below `parts` counts)
   }
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
     mine += __shfl_xor_sync(0xffffffffu, mine, w);
-    items += min(__shfl_xor_sync(0xffffffffu, items, w), parts);  // (only below `parts` counts)
+    items = min(items + __shfl_xor_sync(0xffffffffu, items, w), parts);
   }
   // Little work is not cut into as many pieces as there are CTAs, whose join would cost more
   // than it saves: shares of `least` at least, but four for each item, so that items that are

@@ -566,24 +566,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;  // m in log2 units
       uint32_t parts = 0;            // of the piece so far
       for (int j = jb; j < t1 && ok; j += step) {
-        if ((j + 1) * kTile > kv_len) {  // rows of V behind the last key
-          const uint32_t entry = 2 * (tile0 + j - t0) + 1;
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&bars.kv_full[entry % kStages], entry / kStages & 1));
-          if (ok && j * kTile + r >= kv_len) {
-            const uint32_t row = skv + entry % kStages * kTileBytes + Layout::row(r);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              st_shared_v4(row + 16 * c, 0, 0, 0, 0);
-              st_shared_v4(row + Layout::kHalf + 16 * c, 0, 0, 0, 0);
-            }
-          }
-          fence_proxy_async();
-        }
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t][h], ns & 1));
           if (!ok) break;
+          if (h == 0 && (j + 1) * kTile > kv_len) {
+            // Rows of V behind the last key.  These scores were issued after the values of this
+            // half's tile before, so the stage's earlier tile has long arrived and the wait
+            // below is for this one (before that, its parity would be the one before last's).
+            const uint32_t entry = 2 * (tile0 + j - t0) + 1;
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(&bars.kv_full[entry % kStages], entry / kStages & 1));
+            if (ok && j * kTile + r >= kv_len) {
+              const uint32_t row = skv + entry % kStages * kTileBytes + Layout::row(r);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                st_shared_v4(row + 16 * c, 0, 0, 0, 0);
+                st_shared_v4(row + Layout::kHalf + 16 * c, 0, 0, 0, 0);
+              }
+            }
+            fence_proxy_async();
+            if (!ok) break;
+          }
           tc_fence_after();
           const uint32_t tp = ts + kPart * h;
           float s[2][32];

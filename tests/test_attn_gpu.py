@@ -162,6 +162,23 @@ def test_paged_long_context_is_split_and_joined(cuda, q_len):
         assert torch.equal(out, pkg.attn_paged(*args, cu_seqlens=g["cu"]))
 
 
+@pytest.mark.parametrize("page", [8, 64])
+@pytest.mark.parametrize("q_lens", [[9, 29, 17, 32], [1059, 29, 300, 12]])
+def test_paged_last_tile_of_a_block_of_one_row_tile(cuda, page, q_lens):
+    """Blocks of one row tile, whose key tiles two warp groups take in turn, over contexts that
+    end inside a tile: the values behind the end are zeroed where they arrived, not in the
+    stage's tile before (many small pages make those arrive late)."""
+    pkg = load_pkg()
+    for seed in range(4):
+        kv_lens = [2884, 2884 + seed, 1414, 2500 + 31 * seed]
+        d = paged_inputs(q_lens, kv_lens, 8, 2, page, seed=seed, stale=float("nan"))
+        ref, size = paged_ref(d)
+        g = on(d, cuda)
+        out = pkg.attn_paged(g["q"], g["k_cache"], g["v_cache"], g["table"], g["kv_lens"],
+                             cu_seqlens=g["cu"])
+        check(out, ref, size, f"seed {seed}")
+
+
 @pytest.mark.parametrize("q_len", [1, 40])
 def test_paged_bad_pages_read_as_zeros(cuda, q_len):
     """Page numbers outside the cache (checked on the device, nothing is read for them)."""
