@@ -200,8 +200,11 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
     auto find_page = [&] {  // asked for a chunk ahead of its use
       if (a.paged) page = lkey + mkey + (lane & 15) < lend ? __ldg(ltable + lidx) : -1;
     };
-    // To the next chunk; `n` is the piece at hand (a wait for one kWorks later would not end).
+    // To the next chunk; `n` is the piece at hand (a wait for one kWorks later would not end,
+    // and the place of one before it may hold another by now: a group without chunks in
+    // several pieces on end comes late).
     auto open = [&](uint32_t n) {
+      if (ln < n) ln = n;
       while (!opened && more && ln < n + kWorks) {
         if (!__all_sync(0xffffffffu, mbar_wait(&work_full[ln % kWorks], ln / kWorks & 1))) {
           ok = more = false;
@@ -288,6 +291,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
       }
       const Work& w = works[n % kWorks];
       if (!w.live) break;
+      while (issued < done + kRing - 1 && open(n)) issue();
       // the item's queries, as K and V: 64 columns of all rows, 128-byte swizzle
       for (int i = tid; i < kRowsItem * 16; i += kWarps * 32) {
         const int r = i >> 4, c = i & 15, tok = r / grp;
@@ -328,7 +332,6 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
       const int first = w.k0 + group * kChunk;
       const uint32_t begun = done;
       for (int key0 = first; key0 < w.k1; key0 += kRound) {
-        while (issued < done + kRing - 1 && open(n)) issue();
         // this chunk has arrived: of the loads issued, all but the chunks behind it
         if (kRing == 3 && issued > done + 1)
           asm volatile("cp.async.wait_group 1;" ::: "memory");

@@ -257,6 +257,24 @@ def test_many_sequences(cuda):
     check(pkg.attn_prefill(g["q"], g["k"], g["v"], g["cu"]), ref, size)
 
 
+@pytest.mark.parametrize("hq,hk,q_len", [(8, 8, 1), (16, 8, 1), (16, 2, 2), (16, 2, 4)])
+def test_short_contexts_with_long_ones_between(cuda, hq, hk, q_len):
+    """Runs of contexts too short for some warps to have a chunk, then longer ones: every warp
+    finds its next chunk, however many pieces it had none in."""
+    pkg = load_pkg()
+    n = 700
+    kv_lens = [q_len + ((i * 37) % 90 if i % 11 else 200 + (i * 53) % 500) for i in range(n)]
+    d = paged_inputs([q_len] * n, kv_lens, hq, hk, 16, seed=hq + q_len, stale=float("nan"))
+    ref, size = paged_ref(d)
+    g = on(d, cuda)
+    for _ in range(3):
+        out = pkg.attn_paged(g["q"], g["k_cache"], g["v_cache"], g["table"], g["kv_lens"],
+                             cu_seqlens=g["cu"])
+        torch.cuda.synchronize()
+        assert pkg.device_error() == 0
+        check(out, ref, size)
+
+
 @pytest.mark.parametrize("q_len", [1, 64])
 def test_offsets_beyond_32_bits(cuda, q_len):
     """A cache of more than 2^32 elements in each of K and V: the last pages are read."""
