@@ -83,7 +83,7 @@ cudaError_t launch_attn_tc(const AttnArgs& p, int sms, void* workspace, unsigned
                            cudaStream_t st);
 unsigned read_attn_tc_error(bool clear);
 
-// Kernel for few rows: an item has at most `rows` (8, 16, 32 or 64) of them.
+// Kernel for few rows: an item has at most `rows` (8, 16 or 32) of them.
 cudaError_t launch_attn_rows(const AttnArgs& p, int rows, int sms, void* workspace,
                              unsigned long long tag, cudaStream_t st);
 unsigned read_attn_rows_error(bool clear);

@@ -1,10 +1,9 @@
 // Causal softmax attention for few query rows: decode steps and draft tokens over a paged
 // cache (or very short prompts).  Bound by the HBM traffic of K and V.
 //
-// An item has up to R = 8, 16, 32 or 64 rows: the query heads of one key/value head for as
-// many tokens as fit.  Every SM runs one CTA whose twelve consumer warps split the keys: a
-// group of W warps shares a chunk of 16 W keys, each warp for 8 NT of the rows (R = 8 NT W).
-// Each group has two chunks in shared memory (192 KB a CTA) that its own lanes fill by
+// An item has up to R = 8, 16 or 32 rows: the query heads of one key/value head for as many
+// tokens as fit.  Every SM runs one CTA whose twelve consumer warps split the keys: a group of
+// W = R / 8 warps shares a chunk of 16 W keys, each warp for 8 of the rows.  Each group has two chunks in shared memory (192 KB a CTA) that its own lanes fill by
 // cp.async, the next one while they work, across the ends of pieces; a box of 16 keys is too
 // small for TMA, whose issue then bounds the loads (2 KB boxes measured 5.2 TB/s from eight
 // lanes and 2.0 TB/s from one).
@@ -30,9 +29,11 @@ using namespace sm100;
 
 constexpr int kTile = kAttnTile;
 constexpr int kWorks = 4;   // pieces handed out ahead
-constexpr size_t smem_bytes(int warps, int ring, int rows) {  // ring, queries (later the join's weights)
+constexpr int kWarps = 12;  // that consume
+constexpr int kRing = 2;    // chunks of a group in shared memory
+constexpr size_t smem_bytes(int rows) {  // ring, queries (later the join's weights)
   static_assert(attn_weight_bytes(1) <= kHeadDim * 2, "the weights take the queries' place");
-  return 1024 + (size_t)ring * 16 * warps * 2 * kHeadDim * 2 + (size_t)rows * kHeadDim * 2;
+  return 1024 + (size_t)kRing * 16 * kWarps * 2 * kHeadDim * 2 + (size_t)rows * kHeadDim * 2;
 }
 
 __device__ unsigned int g_rows_error = 0;
@@ -80,7 +81,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-template <int W, int NT, int kWarps, int kRing>
+template <int W>
 __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
     attn_rows_kernel(const __grid_constant__ RowsArgs p) {
   constexpr int kGroups = kWarps / W;
@@ -88,7 +89,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
   constexpr int kChunk = 16 * W;               // keys
   constexpr int kHalf = kChunk * 128;          // 64 columns of a chunk's K or V
   constexpr int kStage = 4 * kHalf;            // K, V
-  constexpr int kRowsItem = 8 * NT * W;
+  constexpr int kRowsItem = 8 * W;
   static_assert(kRowsItem * kHeadDim * 4 <= kStage, "the join goes through a stage");
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t work_full[kWorks], pieces_full[kWorks], work_empty[kWorks];
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
     // ------------------------------------------------------------------ consumers
     const int group = warp / W;
     const int mkey = (warp % W) * 16;              // the chunk's keys that the warp loads
-    const int mrow = (warp % W) * 8 * NT;          // its first row
+    const int mrow = (warp % W) * 8;               // its first row
     const int fr = lane >> 2, fc = 2 * (lane & 3);  // row and column pair of a fragment
     const uint32_t stages = ring0 + group * kRing * kStage;
     uint32_t done = 0;  // chunks consumed
@@ -303,41 +304,26 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
         st_shared_v4(sq + (c >> 3) * kRowsItem * 128 + sw128(r, c & 7), x.x, x.y, x.z, x.w);
       }
       group_sync(1, kWarps * 32);
-      // the thread's rows (columns of the transposed products) are mrow + 8 t + fc and the
-      // next one: keys that they see.  One tile of rows keeps its queries, the B operand, in
-      // registers; two would spill (216 bytes).
-      int lim[NT][2];
+      // the thread's rows (columns of the transposed products) are mrow + fc and the next one:
+      // keys that they see.  The queries, the B operand, stay in registers.
+      int lim[2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int r = mrow + 8 * t + fc + k, tok = r / grp;
-          lim[t][k] = r < g.sub * grp && tok < w.toks ? max(w.lim0 + tok, 0) : 0;
-        }
-      const int qrow = NT == 1 ? mrow + (lane & 7) : mrow + 8 * (lane >> 4) + (lane & 7);
-      uint32_t qk[NT == 1 ? 4 : 1][4];
-      if constexpr (NT == 1) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)  // two steps of 16 columns
-          ldmatrix4(sq + (i >> 1) * kRowsItem * 128 + sw128(qrow, 4 * (i & 1) + (lane >> 3)), qk[i]);
+      for (int k = 0; k < 2; ++k) {
+        const int r = mrow + fc + k, tok = r / grp;
+        lim[k] = r < g.sub * grp && tok < w.toks ? max(w.lim0 + tok, 0) : 0;
       }
-      float o[NT][8][4], m[NT][2], l[NT][2];
+      uint32_t qk[4][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        m[t][0] = m[t][1] = -INFINITY;
-        l[t][0] = l[t][1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
-      }
+      for (int i = 0; i < 4; ++i)  // two steps of 16 columns
+        ldmatrix4(sq + (i >> 1) * kRowsItem * 128 +
+                      sw128(mrow + (lane & 7), 4 * (i & 1) + (lane >> 3)),
+                  qk[i]);
+      float o[8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
       const int first = w.k0 + group * kChunk;
       const uint32_t begun = done;
       for (int key0 = first; key0 < w.k1; key0 += kRound) {
-        // this chunk has arrived: of the loads issued, all but the chunks behind it
-        if (kRing == 3 && issued > done + 1)
-          asm volatile("cp.async.wait_group 1;" ::: "memory");
-        else
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-        static_assert(kRing == 2 || kRing == 3, "one or two chunks are on their way");
+        // this chunk has arrived, the only one on its way
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         if constexpr (W > 1) group_sync(2 + group, W * 32);
         else __syncwarp();
         if (open(n)) issue();  // into the stage of the chunk before, which everyone has left
@@ -345,79 +331,53 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
         ++done;
 #pragma unroll
         for (int c = 0; c < W; ++c) {  // 16 keys
-          float s[NT][4], s2[NT][4];   // two chains of four products
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[t][k] = s2[t][k] = 0.f;
+          float s[4] = {}, s2[4] = {};  // two chains of four products
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             uint32_t kf[4];
             ldmatrix4(kb + (i >> 2) * kHalf + sw128(16 * c + (lane & 15), 2 * (i & 3) + (lane >> 4)),
                       kf);
-            if constexpr (NT == 1) {
-              mma16816((i & 1) ? s2[0] : s[0], kf, qk[i >> 1][2 * (i & 1)],
-                       qk[i >> 1][2 * (i & 1) + 1]);
-            } else {
-              uint32_t qf[4];
-              ldmatrix4(sq + (i >> 2) * kRowsItem * 128 +
-                            sw128(qrow, 2 * (i & 3) + ((lane >> 3) & 1)),
-                        qf);
-              mma16816((i & 1) ? s2[0] : s[0], kf, qf[0], qf[1]);
-              mma16816((i & 1) ? s2[1] : s[1], kf, qf[2], qf[3]);
-            }
+            mma16816((i & 1) ? s2 : s, kf, qk[i >> 1][2 * (i & 1)], qk[i >> 1][2 * (i & 1) + 1]);
           }
-          const int k0 = key0 + 16 * c + fr;  // key of s[.][0], s[.][1]; k0 + 8 of the others
-          bool up = false;
+          const int k0 = key0 + 16 * c + fr;  // key of s[0], s[1]; k0 + 8 of the others
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              s[t][k] = (s[t][k] + s2[t][k]) * a.scale_log2;
-              if (k0 + (k & 2) * 4 >= lim[t][k & 1]) s[t][k] = -INFINITY;
-            }
-            up = up || fmaxf(s[t][0], s[t][2]) > m[t][0] + kRaise ||
-                 fmaxf(s[t][1], s[t][3]) > m[t][1] + kRaise;
+          for (int k = 0; k < 4; ++k) {
+            s[k] = (s[k] + s2[k]) * a.scale_log2;
+            if (k0 + (k & 2) * 4 >= lim[k & 1]) s[k] = -INFINITY;
           }
+          const bool up = fmaxf(s[0], s[2]) > m[0] + kRaise || fmaxf(s[1], s[3]) > m[1] + kRaise;
           if (__any_sync(0xffffffffu, up)) {  // some row's maximum has to be raised
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int k = 0; k < 2; ++k) {
+              float x = fmaxf(s[k], s[k + 2]);
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+              x = fmaxf(x, m[k]);
+              const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - x);
+              m[k] = x;
+              l[k] *= f;
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                float x = fmaxf(s[t][k], s[t][k + 2]);
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                x = fmaxf(x, m[t][k]);
-                const float f = m[t][k] == -INFINITY ? 0.f : ex2(m[t][k] - x);
-                m[t][k] = x;
-                l[t][k] *= f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  o[t][i][k] *= f;
-                  o[t][i][k + 2] *= f;
-                }
+              for (int i = 0; i < 8; ++i) {
+                o[i][k] *= f;
+                o[i][k + 2] *= f;
               }
-          }
-          uint32_t pf[NT][2];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              s[t][k] = ex2(s[t][k] - (m[t][k & 1] == -INFINITY ? 0.f : m[t][k & 1]));
-              l[t][k & 1] += s[t][k];
             }
-            pf[t][0] = transpose8x8(pack_bf16(s[t][0], s[t][1]));
-            pf[t][1] = transpose8x8(pack_bf16(s[t][2], s[t][3]));
           }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            s[k] = ex2(s[k] - (m[k & 1] == -INFINITY ? 0.f : m[k & 1]));
+            l[k & 1] += s[k];
+          }
+          const uint32_t p0 = transpose8x8(pack_bf16(s[0], s[1]));
+          const uint32_t p1 = transpose8x8(pack_bf16(s[2], s[3]));
 #pragma unroll
           for (int i = 0; i < 8; ++i) {  // 16 columns of V
             uint32_t vf[4];
             ldmatrix4_trans(vb + (i >> 2) * kHalf + sw128(16 * c + (lane >> 4) * 8 + (lane & 7),
                                                           2 * (i & 3) + ((lane >> 3) & 1)),
                             vf);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) mma16816(o[t][i], vf, pf[t][0], pf[t][1]);
+            mma16816(o[i], vf, p0, p1);
           }
         }
       }
@@ -427,29 +387,25 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
       const uint32_t last = (done - 1) % kRing;
       if (lane == 0) kept[group] = last;  // the same from each of the group's warps
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float x = l[t][k];
-          x += __shfl_xor_sync(0xffffffffu, x, 4);
-          x += __shfl_xor_sync(0xffffffffu, x, 8);
-          x += __shfl_xor_sync(0xffffffffu, x, 16);
-          if (fr == 0) stat[group][mrow + 8 * t + fc + k] = make_float2(m[t][k], x);
-        }
+      for (int k = 0; k < 2; ++k) {
+        float x = l[k];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (fr == 0) stat[group][mrow + fc + k] = make_float2(m[k], x);
+      }
       if constexpr (W > 1) group_sync(2 + group, W * 32);  // the others have read V
       if (has) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = mrow + 8 * t + fc + (k & 1), d = 16 * i + fr + (k & 2) * 4;
-              asm volatile("st.shared.f32 [%0], %1;" ::"r"(stages + last * kStage + r * 512 +
-                                                           4 * (d ^ ((r >> 1 & 3) << 3))),
-                           "f"(o[t][i][k])
-                           : "memory");
-            }
+          for (int k = 0; k < 4; ++k) {
+            const int r = mrow + fc + (k & 1), d = 16 * i + fr + (k & 2) * 4;
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(stages + last * kStage + r * 512 +
+                                                         4 * (d ^ ((r >> 1 & 3) << 3))),
+                         "f"(o[i][k])
+                         : "memory");
+          }
       }
       if (group_or(1, kWarps * 32, !ok)) {
         ok = false;
@@ -531,13 +487,13 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
   }
 }
 
-template <int W, int NT, int kWarps, int kRing>
+template <int W>
 cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long long tag,
                    cudaStream_t st) {
   const int grp = a.hq / a.hkv;
   RowsArgs p{};
   p.a = a;
-  constexpr int rows = 8 * NT * W;
+  constexpr int rows = 8 * W;
   p.g.sub = rows / grp;
   p.g.block = p.g.sub;
   p.g.overhead = 128;
@@ -550,13 +506,12 @@ cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long lo
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (set_for != dev) {
-    e = cudaFuncSetAttribute(attn_rows_kernel<W, NT, kWarps, kRing>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem_bytes(kWarps, kRing, rows));
+    e = cudaFuncSetAttribute(attn_rows_kernel<W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem_bytes(rows));
     if (e != cudaSuccess) return e;
     set_for = dev;
   }
-  attn_rows_kernel<W, NT, kWarps, kRing>
-      <<<sms, (kWarps + 1) * 32, smem_bytes(kWarps, kRing, rows), st>>>(p);
+  attn_rows_kernel<W><<<sms, (kWarps + 1) * 32, smem_bytes(rows), st>>>(p);
   return cudaGetLastError();
 }
 
@@ -574,9 +529,9 @@ unsigned read_attn_rows_error(bool clear) {
 
 cudaError_t launch_attn_rows(const AttnArgs& p, int rows, int sms, void* workspace,
                              unsigned long long tag, cudaStream_t st) {
-  return rows == 8    ? launch<1, 1, 12, 2>(p, sms, workspace, tag, st)
-         : rows == 16 ? launch<2, 1, 12, 2>(p, sms, workspace, tag, st)
-                      : launch<4, 1, 12, 2>(p, sms, workspace, tag, st);
+  return rows == 8    ? launch<1>(p, sms, workspace, tag, st)
+         : rows == 16 ? launch<2>(p, sms, workspace, tag, st)
+                      : launch<4>(p, sms, workspace, tag, st);
 }
 
 }  // namespace gdn
