@@ -453,8 +453,9 @@ int gdn_attn_qk_norm_rope_launch(const void* q, const void* k, const void* v,
                                  long long q_out_stride, long long k_out_stride, void* stream);
 
 /*
- * Bytes of device workspace the two attention entry points below need (may be 0); 16-byte
- * aligned scratch, not shared by calls that overlap on the GPU.
+ * Bytes of device workspace that the two attention entry points below need (0 where there is
+ * nothing to do); 16-byte aligned scratch, whatever it holds, not shared by calls that
+ * overlap on the GPU.
  */
 size_t gdn_attn_workspace_size(int total_q, int num_seqs, int num_q_heads, int num_kv_heads);
 

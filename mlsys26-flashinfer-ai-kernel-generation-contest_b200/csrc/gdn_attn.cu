@@ -36,14 +36,23 @@ int parts() {
   return n;
 }
 
-// Rows of an item for the few-rows kernel, or 0 where the tensor-core kernel runs.
-int few_rows(long long total_q, int num_seqs, int hq, int hkv) {
-  const long long rows = (total_q + num_seqs - 1) / num_seqs * (hq / hkv);
-  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
+// Rows of an item for the few-rows kernel, or 0 where the tensor-core kernel runs.  Up to 32
+// rows on average the former's padding and hand-overs are the smaller (64 single tokens of 4096
+// keys, 16 / 2 heads: 55 us, the other 92; 32 x 4: 53 and 58).  The host does not see how
+// ragged a packed batch is.  One chunk among single tokens would be read by many small items,
+// so past 32 items in the longest sequence that is possible the tensor cores take it (255
+// single tokens and a chunk of 512 over 16384 keys, 8 / 8 heads: 329 us, few rows 604; below,
+// 63 and a chunk of 256 over 8192: few rows 219, the other 295).
+int few_rows(long long total_q, int num_seqs, int hq, int hkv, bool uniform) {
+  const int grp = hq / hkv;
+  const long long mean = (total_q + num_seqs - 1) / num_seqs * grp;
+  const int rows = mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 32 ? 32 : 0;
+  return !uniform && (total_q - num_seqs) * grp > 32 * rows ? 0 : rows;
 }
 
+// (It does not depend on how the tokens come: of the larger of the two choices.)
 size_t workspace_size(long long total_q, int num_seqs, int hq, int hkv) {
-  const int few = few_rows(total_q, num_seqs, hq, hkv);
+  const int few = few_rows(total_q, num_seqs, hq, hkv, false);
   return attn_workspace_bytes(few ? few : attn_tc_rows(), kAttnMaxParts);
 }
 
@@ -64,7 +73,7 @@ int launch(AttnArgs& p, float scale, void* workspace, size_t workspace_bytes, vo
     return GDN_ERR_WORKSPACE;
   if (misaligned(workspace, 16)) return GDN_ERR_INVALID_ARGUMENT;
   p.scale_log2 = default_scale(scale) * 1.4426950408889634f;
-  const int few = few_rows(p.total_q, p.num_seqs, p.hq, p.hkv);
+  const int few = few_rows(p.total_q, p.num_seqs, p.hq, p.hkv, p.cu == nullptr);
   const unsigned long long tag = next_tag();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = few ? launch_attn_rows(p, few, parts(), workspace, tag, st)

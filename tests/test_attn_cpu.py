@@ -65,6 +65,31 @@ def test_entry_points_refuse_before_launch(call, bad, unsupported):
     assert call(t=0) == 0  # nothing to do
 
 
+@pytest.mark.parametrize("t,n,hq,hk", [(1, 1, 1, 1), (10, 1, 8, 2), (10, 2, 8, 2), (64, 64, 8, 2),
+                                       (128, 32, 8, 2), (5000, 3, 64, 1), (1500, 1000, 2, 2)])
+def test_workspace(t, n, hq, hk):
+    """The size is enough for either form of a call: one byte less, none or a misaligned one is
+    refused (and with the whole of it the next refusal comes first: alignment)."""
+    need = load_pkg().LIB.gdn_attn_workspace_size(t, n, hq, hk)
+    assert need > 0
+    kw = dict(t=t, n=n, hq=hq, hk=hk, qs=hq * 128, os=hq * 128)
+    calls = [(prefill_call, dict(kw, ks=hk * 128, vs=hk * 128)),
+             (paged_call, dict(kw, kps=16 * hk * 128, vps=16 * hk * 128))]
+    if t % n == 0:
+        calls.append((paged_call, dict(calls[1][1], cu=None)))
+    for call, a in calls:
+        assert call(**a, ws=None, wsb=need) == -4
+        assert call(**a, ws=FAKE, wsb=0) == -4
+        assert call(**a, ws=FAKE, wsb=need - 1) == -4
+        assert call(**a, ws=FAKE + 8, wsb=need) == -1
+
+
+@pytest.mark.parametrize("bad", [(0, 1, 8, 2), (-3, 1, 8, 2), (10, 0, 8, 2), (10, 1, 8, 0),
+                                 (10, 1, 1, 2), (10, 1, 0, 0)])
+def test_workspace_of_nothing(bad):
+    assert load_pkg().LIB.gdn_attn_workspace_size(*bad) == 0
+
+
 def test_host_functions_refuse_cpu_tensors():
     pkg = load_pkg()
     d = prefill_inputs([4], 4, 2, seed=0)

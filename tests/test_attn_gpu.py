@@ -273,6 +273,31 @@ def test_short_contexts_with_long_ones_between(cuda, hq, hk, q_len):
         torch.cuda.synchronize()
         assert pkg.device_error() == 0
         check(out, ref, size)
+        x = g["q"].view(n, q_len, hq, D)  # the same number of tokens each: known to the host
+        out = pkg.attn_paged(x, g["k_cache"], g["v_cache"], g["table"], g["kv_lens"])
+        torch.cuda.synchronize()
+        assert pkg.device_error() == 0
+        check(out, ref, size)
+
+
+@pytest.mark.parametrize("hq,hk,chunk", [(2, 2, 200), (2, 2, 300), (16, 2, 30), (16, 2, 140)])
+def test_a_chunk_among_many_single_tokens(cuda, hq, hk, chunk):
+    """Few tokens a sequence on average, on both sides of the longest chunk for which the
+    kernel for few rows is taken."""
+    pkg = load_pkg()
+    q_lens = [1] * 90 + [chunk] + [1] * 60
+    d = paged_inputs(q_lens, [x + (17 * i) % 150 for i, x in enumerate(q_lens)], hq, hk, 16,
+                     seed=chunk, stale=float("nan"))
+    ref, size = paged_ref(d)
+    g = on(d, cuda)
+    check(pkg.attn_paged(g["q"], g["k_cache"], g["v_cache"], g["table"], g["kv_lens"],
+                         cu_seqlens=g["cu"]), ref, size)
+    d = prefill_inputs(q_lens, hq, hk, seed=chunk + 1)
+    ref, size = A.prefill(d["q"], d["k"], d["v"], d["cu"])
+    g = on(d, cuda)
+    check(pkg.attn_prefill(g["q"], g["k"], g["v"], g["cu"]), ref, size)
+    torch.cuda.synchronize()
+    assert pkg.device_error() == 0
 
 
 @pytest.mark.parametrize("q_len", [1, 64])
