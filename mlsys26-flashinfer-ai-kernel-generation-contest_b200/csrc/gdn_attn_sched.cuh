@@ -6,9 +6,9 @@
 // in the order (sequence, head, block), lie on one line that is cut into one equal range
 // per CTA: ragged batches, causal blocks and one long sequence come out balanced alike,
 // and no list is made.  A cut inside an item splits its keys, at a tile; both sides write
-// partial results, and a second kernel joins the pieces in the order of the keys (so the
-// result does not depend on timing).  An item of few tiles is not split: it goes to the
-// CTA that holds its middle.
+// partial results, and the CTA that finishes last joins the pieces in the order of the keys
+// (so the result does not depend on timing).  An item of few tiles is not split: it goes to
+// the CTA that holds its middle.
 #pragma once
 
 #include "gdn_attn.cuh"
@@ -225,34 +225,32 @@ inline AttnPartials attn_partials(void* workspace, int rows, unsigned long long 
                       reinterpret_cast<float*>(static_cast<AttnCounters*>(workspace) + 1), tag,
                       rows};
 }
-// A counter's memory may hold anything before the first arrival: only a word with this
-// launch's tag counts.  The first arrival puts it there; whoever finds that done just adds,
-// so that no arrival waits for others' (a loop of compare-and-swaps by 16 CTAs that finish
-// together took 8 us).  The last of n arrivals (true) clears the word, for the next replay
-// of a captured launch, whose tag is the same.
-__device__ __forceinline__ bool attn_arrive(unsigned long long* word, unsigned long long tag,
-                                            int n) {
-  const unsigned long long first = (tag << 16) | 1;
-  unsigned long long seen = 0, was = atomicCAS(word, seen, first);  // cleared by an earlier launch?
-  if (was != seen && (was >> 16) != tag) {
-    seen = was;
-    was = atomicCAS(word, seen, first);
-  }
-  int k = 1;
-  if (was != seen) k = (int)(atomicAdd(word, 1ull) & 0xffffu) + 1;  // it has the tag
-  if (k == n) atomicExch(word, 0ull);
-  return k == n;
+// A counter's memory may hold anything before the launch: only a word with this launch's tag
+// counts.  Each CTA of an item sees to the tag well before it arrives (attn_pieces), so that an
+// arrival is one addition (a loop of compare-and-swaps by 16 CTAs that finish together took
+// 8 us).  The last of n arrivals (true) clears the word; no CTA tags it after that, since each
+// does so before its own arrival.
+__device__ __forceinline__ void attn_tag(unsigned long long* word, unsigned long long tag) {
+  const unsigned long long was = atomicCAS(word, 0ull, tag << 16);  // cleared by an earlier launch?
+  if (was != 0 && (was >> 16) != tag) atomicCAS(word, was, tag << 16);  // (or another CTA was first)
 }
+__device__ __forceinline__ bool attn_arrive(unsigned long long* word, int n) {
+  const bool last = (int)(atomicAdd(word, 1ull) & 0xffffu) + 1 == n;
+  if (last) atomicExch(word, 0ull);
+  return last;
+}
+__device__ __forceinline__ void attn_fence() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 
 // The pieces of one item, in the order of the keys, as every one of its CTAs finds them.
 struct AttnPieces {
   short list[kAttnMaxParts];  // 2 CTA + slot
   int count, mine;            // mine: this CTA's place in the list
 };
-// By one warp, for the item `cur` (e keys, n tiles) and CTA `cta`.
+// By one warp, for the item at cost `start` (e keys, n tiles) and CTA `cta`; tags the counters
+// that this CTA may arrive at, for `tiles` row tiles.
 __device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& line,
-                                            long long start, int e, int n, int cta,
-                                            AttnPieces* out) {
+                                            const AttnPartials& ws, long long start, int e, int n,
+                                            int cta, int tiles, AttnPieces* out) {
   const int lane = threadIdx.x & 31;
   const long long end = start + e + g.overhead;
   int count = 0;
@@ -276,6 +274,12 @@ __device__ __forceinline__ void attn_pieces(const AttnGrid& g, const AttnLine& l
     count += __popc(some);
   }
   if (lane == 0) out->count = count;
+  __syncwarp();
+  const int level = lane >> 1, tile = lane & 1;
+  if (level < (count > kAttnFan ? 2 : 1) && tile < tiles) {
+    const int first = level == 0 ? out->mine / kAttnFan * kAttnFan : 0;
+    attn_tag(&ws.counters->arrived[out->list[first]][level][tile], ws.tag);
+  }
 }
 
 // Joins `count` <= kAttnFan pieces list[0], list[step], .. of the rows [row0, row0 + rows),
@@ -365,9 +369,9 @@ __device__ __forceinline__ void attn_join(const AttnPartials& ws, const AttnPiec
   auto arrive = [&](int first, int level, int n) {  // true in the last CTA to arrive
     sync();  // the others' rows before this thread's fence
     if (warp == 0 && lane == 0) {
-      __threadfence();
-      *flag = attn_arrive(&ws.counters->arrived[pieces.list[first]][level][tile], ws.tag, n);
-      __threadfence();
+      attn_fence();
+      *flag = attn_arrive(&ws.counters->arrived[pieces.list[first]][level][tile], n);
+      attn_fence();
     }
     sync();
     return *flag != 0;

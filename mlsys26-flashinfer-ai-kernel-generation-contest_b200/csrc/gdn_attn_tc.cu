@@ -3,13 +3,22 @@
 //   S = scale Q K^T,  P = 2^(S - m),  l = sum P,  O = P V / l
 // over tiles of 128 keys with a running maximum m per row.  A tile of 128 rows holds the
 // query heads of one key/value head for 128 / group tokens (all of them read the same keys),
-// and a CTA works on two such tiles, in turn: while one's scores go through the exponential
-// (16 per clock and SM), the tensor cores multiply for the other.
+// and a CTA works on two such tiles: while one's scores go through the exponential (16 per
+// clock and SM), the tensor cores multiply for the other.  A row's scores are taken 64 keys at
+// a time, into two buffers, so that a tile's next product never waits for its own softmax.  A
+// block of one tile of rows ("twin") gives its key tiles to both halves of the CTA in turn,
+// whose results are merged at the end.
 //
 // Warps 0-3 and 4-7: softmax of tile 0 and 1, one row per thread, scores read from TMEM and
-// P written back over them as the bf16 A operand of the second product.  Warp 8: issues the
-// products.  Warp 9: loads K and V tiles by TMA into a ring of four (K and V in turn), Q once
-// per item.  (Warps 10 and 11 fill the register group.)  TMEM: S0 S1 O0 O1, 128 columns each.
+// P written back over them as the bf16 A operand of the second product.  Warps 8 and 11: issue
+// the products of tile 0 and 1.  Warp 9: loads K and V tiles by TMA into a ring of four (K and
+// V in turn), Q once per item.  Warp 10: finds the pieces of work, two ahead.  TMEM: S0 S1 O0
+// O1, 128 columns each.
+//
+// Bound by the softmax warps, with the tensor pipe close behind: a tile pair of 128 x 128
+// scores takes 4 x 64 x 8 clocks of products and 2 x 1024 of exponentials, of which a quarter
+// goes to the FMA pipe.  One prompt of 16384 tokens (16 / 2 heads): 0.91 to 0.99 ms, 1.1 to 1.2
+// PFLOP/s, by the clock that the power limit leaves (cuBLAS: 1.68).
 //
 // The maximum that a row's sums are relative to is raised only when the new one exceeds it
 // by 2^8: P then stays below 2^8 and the sums in fp32 lose nothing, and the rescaling of O
@@ -44,7 +53,7 @@ struct Bars {
   uint64_t q_full[2], q_empty;
   uint64_t kv_full[kStages], kv_empty[kStages];
   uint64_t s_full[2][2], p_ready[2][2], pv_done[2], o_full[2];
-  uint64_t work_full[kWorks], work_empty[kWorks];
+  uint64_t work_full[kWorks], pieces_full[kWorks], work_empty[kWorks];
   uint64_t twin_ready, twin_done;
   uint64_t drain[2];
 };
@@ -80,9 +89,9 @@ struct TcArgs {
   int box;  // key rows per TMA box
 };
 
-// The piece of item `cur` inside [u0, u1); false if there is none.
-// (By a whole warp; lane 0 writes it.)
-__device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& g,
+// The piece of item `cur` inside [u0, u1), written by lane 0 of a whole warp.
+enum PieceOf { kNone, kWhole, kPartial };
+__device__ __forceinline__ PieceOf piece_of(const AttnCursor& cur, const AttnGrid& g,
                                          const AttnShare& share, Work* w) {
   const long long u0 = share.u0, u1 = share.u1;
   const int e = cur.keys(g);
@@ -90,10 +99,10 @@ __device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& 
   const int t0 = attn_tile_at(g, e, n, u0 > cur.start ? u0 - cur.start : 0);
   const int t1 = attn_tile_at(g, e, n, u1 - cur.start);
   // an item without keys belongs to the CTA that it starts in (its rows are zeroed)
-  if (t1 <= t0 && !(n == 0 && cur.start >= u0)) return false;
+  if (t1 <= t0 && !(n == 0 && cur.start >= u0)) return kNone;
   const int slot = (t0 == 0 && t1 == n) ? -1 : (u0 > cur.start ? 0 : 1);
-  if (slot >= 0) attn_pieces(g, share.line, cur.start, e, n, blockIdx.x, &w->pieces);
-  if ((threadIdx.x & 31) != 0) return true;
+  const PieceOf found = slot < 0 ? kWhole : kPartial;
+  if ((threadIdx.x & 31) != 0) return found;
   const int first = cur.b * g.block;
   w->row0 = cur.seq.q0 + first;
   w->seq = cur.s;
@@ -113,7 +122,7 @@ __device__ __forceinline__ bool piece_of(const AttnCursor& cur, const AttnGrid& 
   w->slot = slot;
   w->twin = w->toks <= g.sub;
   w->live = true;
-  return true;
+  return found;
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -282,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kWorks; ++i) {
       mbar_init(&b.work_full[i], 1);
+      mbar_init(&b.pieces_full[i], 1);
       mbar_init(&b.work_empty[i], 11);  // loader, two issuers, eight softmax warps
     }
     mbar_init(&b.twin_ready, 4);
@@ -319,15 +329,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         if (__any_sync(0xffffffffu, *failed)) break;
         Work* w = &sh.work[n % kWorks];
-        bool found = false;
-        while (more && !found) {
+        PieceOf found = kNone;
+        long long start = 0;
+        int keys = 0, toks = 0;
+        while (more && found == kNone) {
           found = piece_of(cur, g, share, w);
+          start = cur.start;
+          keys = cur.keys(g);
+          toks = cur.seq.q_len - cur.b * g.block;
           more = cur.next(a, g) && cur.start < share.u1;
         }
-        if (lane == 0 && !found) w->live = false;
+        if (lane == 0 && found == kNone) w->live = false;
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.work_full[n % kWorks]);
-        if (!found) break;
+        if (found == kNone) break;
+        // needed at the piece's end only
+        if (found == kPartial)
+          attn_pieces(g, share.line, p.ws, start, keys, (keys + kTile - 1) / kTile, blockIdx.x,
+                      toks > g.sub ? 2 : 1, &w->pieces);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.pieces_full[n % kWorks]);
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------------ loads
@@ -757,6 +778,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int toks = min(w.toks - t * g.sub, g.sub);
         if (slot >= 0 && toks > 0) {
+          // (the entry is not used again before this warp hands it back, so the wait is for
+          // this piece's phase, whatever others it left out)
+          if (!__all_sync(0xffffffffu, mbar_wait(&bars.pieces_full[n % kWorks], n / kWorks & 1)))
+            ok = false;
+          if (group_or(1 + t, 128, !ok)) {
+            ok = false;
+            break;
+          }
           const long long out0 = w.row0 + t * g.sub;
           attn_join<4, 8, 2>(
               p.ws, w.pieces, t, t * kRows, toks * grp, warp & 3, &sh.joining[t],
