@@ -15,10 +15,11 @@
 // V in turn), Q once per item.  Warp 10: finds the pieces of work, two ahead.  TMEM: S0 S1 O0
 // O1, 128 columns each.
 //
-// Bound by the softmax warps, with the tensor pipe close behind: a tile pair of 128 x 128
-// scores takes 4 x 64 x 8 clocks of products and 2 x 1024 of exponentials, of which a quarter
-// goes to the FMA pipe.  One prompt of 16384 tokens (16 / 2 heads): 0.91 to 0.99 ms, 1.1 to 1.2
-// PFLOP/s, by the clock that the power limit leaves (cuBLAS: 1.68).
+// Bound by the chain of each row tile, scores -> TMEM read -> maximum -> exponentials -> P ->
+// product, of which two are in flight: for 128 keys of both tiles the products take 2048 clocks
+// and the exponentials 2048 (16 a clock; 1536 with a quarter of them on the FMA pipe), and the
+// pipes are 55 % and 45 % busy.  One prompt of 16384 tokens (16 / 2 heads): 0.93 to 0.99 ms by
+// the clock that the power limit leaves, 1.1 to 1.2 PFLOP/s (cuBLAS 1.68).
 //
 // The maximum that a row's sums are relative to is raised only when the new one exceeds it
 // by 2^8: P then stays below 2^8 and the sums in fp32 lose nothing, and the rescaling of O
