@@ -20,6 +20,7 @@ namespace gdn {
 constexpr int kAttnSlots = 2;
 constexpr int kAttnTile = 128;      // keys per tile
 constexpr int kAttnMaxParts = 152;  // CTAs that share the work (one per SM)
+constexpr int kAttnFan = 16;        // pieces that one CTA joins; more are joined in two levels
 
 struct AttnGrid {
   int block;     // query tokens per item
@@ -28,6 +29,7 @@ struct AttnGrid {
   int whole;     // items of at most this many tiles are not split
   int snap;      // a cut nearer to an item's end than this many tiles goes to the end
   int least;     // cost below which a CTA's share is not worth a split
+  int each;      // pieces of an item that are, all the same, where there are few items
 };
 
 // Quotients of costs: 32 bits where they do (a 64-bit division is some 100 instructions).
@@ -156,12 +158,12 @@ __device__ __forceinline__ AttnShare attn_share(const AttnArgs& p, const AttnGri
     mine += __shfl_xor_sync(0xffffffffu, mine, w);
     items = min(items + __shfl_xor_sync(0xffffffffu, items, w), parts);
   }
-  // Little work is not cut into as many pieces as there are CTAs, whose join would cost more
-  // than it saves: shares of `least` at least, but four for each item, so that items that are
-  // not split find a CTA each.
-  if (4 * items < parts) {
+  // Little work is not cut into as many pieces as there are CTAs, whose join would cost more than
+  // it saves: shares of `least` at least, but `each` for each item (so items that are not split
+  // find a CTA each).
+  if (g.each * items < parts) {
     const long long some = attn_div(mine, g.least);
-    parts = some < 4 * items ? 4 * items : some < parts ? (int)some : parts;
+    parts = some < g.each * items ? g.each * items : some < parts ? (int)some : parts;
     if (parts < 1) parts = 1;
   }
   r.line.total = mine;
@@ -200,7 +202,6 @@ __device__ __forceinline__ AttnShare attn_share(const AttnArgs& p, const AttnGri
 // ---------------------------------------------------------------- partial results
 // Workspace: arrival counters, then for every CTA and slot the rows of 128 fp32 sums and
 // (maximum in log2 units, sum) of each row.
-constexpr int kAttnFan = 16;  // pieces that one CTA joins; more are joined in two levels
 struct AttnCounters {
   unsigned long long arrived[kAttnMaxParts * kAttnSlots][2][2];  // [first piece][level][row tile]
 };
