@@ -363,6 +363,50 @@ def test_graph_replay_follows_the_lengths(cuda, q_len):
             check(out, ref, size, str(lens))
 
 
+def test_graphs_that_share_memory(cuda):
+    """Several calls in one graph, and two graphs of one memory pool replayed in turn, use the
+    same scratch one after the other: every replay gives the eager calls' results."""
+    pkg = load_pkg()
+    p = on(prefill_inputs([1500, 3, 700], 8, 2, seed=30), cuda)
+    sets = [on(paged_inputs([n] * 3, [5000, 900, 17 + n], 8, 2, 16, seed=31 + n), cuda)
+            for n in (1, 3, 50)]
+
+    def paged(g):
+        return pkg.attn_paged(g["q"], g["k_cache"], g["v_cache"], g["table"], g["kv_lens"],
+                              cu_seqlens=g["cu"])
+    first = lambda: [pkg.attn_prefill(p["q"], p["k"], p["v"], p["cu"])] + [paged(g) for g in sets]  # noqa: E731
+    second = lambda: [paged(g) for g in reversed(sets)]  # noqa: E731
+    want = [[x.clone() for x in f()] for f in (first, second)]
+    torch.cuda.synchronize()
+    pool, graphs, got = torch.cuda.graph_pool_handle(), [], []
+    for f in (first, second):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            got.append(f())
+        graphs.append(graph)
+    for _ in range(4):
+        for i in (0, 1, 1, 0):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            for x, y in zip(want[i], got[i]):
+                assert torch.equal(x, y)
+    assert pkg.device_error() == 0
+
+
+@pytest.mark.parametrize("q_len", [1, 4, 40])
+def test_pages_shared_by_sequences(cuda, q_len):
+    """A prefix whose pages stand in several tables, and a page twice in one."""
+    pkg = load_pkg()
+    n, page = 5, 16
+    d = paged_inputs([q_len] * n, [700 + 9 * i for i in range(n)], 8, 2, page, seed=40 + q_len)
+    d["table"][:, :20] = d["table"][0, :20].clone()
+    d["table"][1, 30] = d["table"][1, 29]
+    ref, size = paged_ref(d, 0.07)
+    g = on(d, cuda)
+    check(pkg.attn_paged(g["q"], g["k_cache"], g["v_cache"], g["table"], g["kv_lens"], 0.07,
+                         cu_seqlens=g["cu"]), ref, size)
+
+
 def test_two_streams_at_once(cuda):
     pkg = load_pkg()
     ds = [prefill_inputs([900 + 100 * i, 40], 4, 2, seed=20 + i) for i in range(3)]
