@@ -120,7 +120,6 @@ def _run(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k_weight,
                                k_weight, qo, ko))
     except (AttributeError, TypeError):
         plan = None
-    eps = float(eps)
     if plan is not None and C.current_device() == plan[-1].index and 0.0 <= eps < math.inf:
         qp, kp, op = q.data_ptr(), k.data_ptr(), qo.data_ptr()
         wq = 0 if q_weight is None else q_weight.data_ptr()
@@ -154,6 +153,7 @@ def _run_checked(q, k, v, positions, table, slots, k_cache, v_cache, q_weight, k
     rd = table.shape[1]
     if rd < 2 or rd > D or rd % 2:
         raise ValueError(f"rope_table must have an even 2..{D} columns, got {rd}")
+    eps = float(eps)
     if not (0.0 <= eps < math.inf):
         raise ValueError(f"eps must be >= 0 and finite, got {eps}")
     given = (q, k, v, q_weight, k_weight)
