@@ -143,8 +143,8 @@ def attn_paged(q, k_cache, v_cache, block_table, kv_lens, scale=None, output=Non
     page_size, HK, 128] (page_size a multiple of 8; pages may be strided); ``block_table``
     int32 [num_seqs, width]: the pages of each sequence in order; ``kv_lens`` int32 or int64
     [num_seqs]: tokens in the cache, the new ones included.  Token i of q_len sees the first
-    kv_len - q_len + i + 1 of them; one that sees none gets zeros.  Returns ``output`` in
-    q's shape; rows behind the last sequence are not written.
+    kv_len - q_len + i + 1 of them; one that sees none, or all of whose scores are -inf (as in
+    :func:`attn_prefill`), gets zeros.  Returns ``output`` in q's shape; rows behind the last sequence are not written.
 
     A page number outside the cache reads as zeros (nothing is read there), a kv_len above
     width * page_size counts as that.  What lies behind kv_len in a page is not used,

@@ -690,7 +690,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = top;
         }
         const bool both = twin && t1 > t0 + 1;      // O_1 holds something
-        const bool saw = mine && lim > t0 * kTile;  // some key of the piece
+        // some key of the piece; of one whose scores are all -inf the sum is 0: zeros too
+        const bool saw = mine && lim > t0 * kTile && l != 0.f;
         auto load = [&](int c, float(&o)[32]) {     // 32 columns of the row's sums, asked for
           if (has) tmem_ld32(to + 32 * c, o);
         };
