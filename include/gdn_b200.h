@@ -500,7 +500,10 @@ int gdn_attn_paged_launch(const void* q, const void* k_cache, const void* v_cach
  * stage of the streaming decode kernel was never released, 16 = the wait of
  * gdn_selftest_bounded_wait ran out; -1 = the device reported an error).  Every wait inside the kernels is bounded; a wait that runs out sets
  * a bit, the kernel releases its resources and returns instead of hanging.
- * The bits are cleared when `clear` != 0.  No counterpart in the reference.
+ * The bits are cleared when `clear` != 0.  What was computed between the failure and the
+ * call that clears its bit is not to be used; afterwards every call works again, and so does
+ * the replay of a captured graph, whatever the failed launch left in its scratch.  Other host
+ * threads must not launch while the bits are cleared.  No counterpart in the reference.
  */
 int gdn_device_error(int clear);
 

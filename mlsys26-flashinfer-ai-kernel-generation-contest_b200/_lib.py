@@ -113,5 +113,7 @@ def check(where: str, status: int) -> None:
 def device_error(clear: bool = True) -> int:
     """Synchronise the current device and return the kernels' device-side error bits
     (0 = none; 1 = a TMA wait ran out; 2 = a tensor-core wait ran out; 8 = a streaming
-    stage was never released; 16 = the self-test's wait ran out)."""
+    stage was never released; 16 = the self-test's wait ran out).  What was computed between a
+    failure and the call that clears its bit is not to be used; other threads must not launch
+    meanwhile."""
     return int(LIB.gdn_device_error(int(bool(clear))))

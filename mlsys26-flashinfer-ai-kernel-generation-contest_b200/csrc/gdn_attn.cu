@@ -56,7 +56,7 @@ size_t workspace_size(long long total_q, int num_seqs, int hq, int hkv) {
   return attn_workspace_bytes(few ? few : attn_tc_rows(), kAttnMaxParts);
 }
 
-// A launch's tag (48 bits, not 0), which memory that was not written by it holds by a chance
+// A call's tag (48 bits, not 0), which memory that was not written by it holds by a chance
 // of 2^-48: a counter mixed by the finaliser of the splitmix64 generator.
 unsigned long long next_tag() {
   static std::atomic<unsigned long long> count{
@@ -136,6 +136,7 @@ bool attn_key_maps(CUtensorMap* mk, CUtensorMap* mv, const AttnArgs& p, int box)
 unsigned read_attn_device_error(bool clear) {
   return read_attn_tc_error(clear) | read_attn_rows_error(clear);
 }
+bool count_attn_report() { return count_attn_tc_report() && count_attn_rows_report(); }
 
 }  // namespace gdn
 

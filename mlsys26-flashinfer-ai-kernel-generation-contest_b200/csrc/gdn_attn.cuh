@@ -77,7 +77,7 @@ bool attn_key_maps(CUtensorMap* mk, CUtensorMap* mv, const AttnArgs& p, int box)
 int attn_key_box(const AttnArgs& p, int most);
 
 // Tensor-core kernel on `sms` CTAs (workspace: attn_workspace_bytes(attn_tc_rows(), sms));
-// `tag`: 48 bits, not 0, another one for every launch.
+// `tag`: 48 bits, not 0, another one for every call (a graph's replays repeat its call's).
 int attn_tc_rows();
 cudaError_t launch_attn_tc(const AttnArgs& p, int sms, void* workspace, unsigned long long tag,
                            cudaStream_t st);
@@ -87,5 +87,10 @@ unsigned read_attn_tc_error(bool clear);
 cudaError_t launch_attn_rows(const AttnArgs& p, int rows, int sms, void* workspace,
                              unsigned long long tag, cudaStream_t st);
 unsigned read_attn_rows_error(bool clear);
+
+// After a failure was read and cleared, with nothing running: what launches that failed left in
+// their scratch counts for no later launch, replays of the same graph among them.
+bool count_attn_tc_report();
+bool count_attn_rows_report();
 
 }  // namespace gdn

@@ -37,6 +37,7 @@ constexpr size_t smem_bytes(int rows) {  // ring, queries (later the join's weig
 }
 
 __device__ unsigned int g_rows_error = 0;
+__device__ unsigned int g_rows_reports = 0;  // of failures, so far (attn_launch_tag)
 
 struct RowsArgs {
   AttnArgs a;
@@ -118,6 +119,8 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
 
   if (warp == kWarps) {
     // ------------------------------------------------------------------ the pieces
+    AttnPartials ws = p.ws;
+    ws.tag = attn_launch_tag(ws.tag, g_rows_reports);
     const AttnShare share = attn_share(a, g, blockIdx.x, gridDim.x);
     const long long u0 = share.u0, u1 = share.u1;
     AttnCursor cur;
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__((kWarps + 1) * 32, 1)
       if (!found) break;
       // needed at the piece's end only
       if (split)
-        attn_pieces(g, share.line, p.ws, start, keys, (keys + kTile - 1) / kTile, blockIdx.x, 1,
+        attn_pieces(g, share.line, ws, start, keys, (keys + kTile - 1) / kTile, blockIdx.x, 1,
                     &w->pieces);
       __syncwarp();
       if (lane == 0) mbar_arrive(&pieces_full[n % kWorks]);
@@ -542,6 +545,13 @@ cudaError_t launch(const AttnArgs& a, int sms, void* workspace, unsigned long lo
 }
 
 }  // namespace
+
+bool count_attn_rows_report() {
+  unsigned v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_rows_reports, sizeof(v)) != cudaSuccess) return false;
+  ++v;
+  return cudaMemcpyToSymbol(g_rows_reports, &v, sizeof(v)) == cudaSuccess;
+}
 
 unsigned read_attn_rows_error(bool clear) {
   unsigned v = 0;

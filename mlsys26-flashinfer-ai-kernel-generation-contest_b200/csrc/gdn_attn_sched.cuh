@@ -212,7 +212,7 @@ __host__ __device__ inline size_t attn_workspace_bytes(int rows, int parts) {
 struct AttnPartials {
   AttnCounters* counters;
   float* base;
-  unsigned long long tag;  // of this launch: 48 bits, not 0
+  unsigned long long tag;  // of this launch: 48 bits, not 0 (attn_launch_tag)
   int rows;
   __device__ __forceinline__ float* sums(int piece) const {  // piece = 2 CTA + slot
     return base + (long long)piece * rows * (kHeadDim + 2);
@@ -225,6 +225,15 @@ inline AttnPartials attn_partials(void* workspace, int rows, unsigned long long 
   return AttnPartials{static_cast<AttnCounters*>(workspace),
                       reinterpret_cast<float*>(static_cast<AttnCounters*>(workspace) + 1), tag,
                       rows};
+}
+// The tag of a launch: the host's, another one for every call, and how many failures have been
+// reported on this device.  A captured graph replays its call's tag; its words are cleared by
+// each replay's last arrivals, but not where a bounded wait ran out: such a replay leaves words
+// of partial counts behind, which the replays after the report are not to take for their own.
+__device__ __forceinline__ unsigned long long attn_launch_tag(unsigned long long tag,
+                                                              unsigned reported) {
+  tag = (tag + reported) & 0xffffffffffffull;
+  return tag != 0 ? tag : 1;
 }
 // A counter's memory may hold anything before the launch: only a word with this launch's tag
 // counts.  Each CTA of an item sees to the tag well before it arrives (attn_pieces), so that an

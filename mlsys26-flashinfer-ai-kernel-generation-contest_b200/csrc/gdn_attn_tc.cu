@@ -48,6 +48,7 @@ constexpr int kThreads = 384;          // 168 registers a thread at launch: 6451
 constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 
 __device__ unsigned int g_attn_error = 0;
+__device__ unsigned int g_attn_reports = 0;  // of failures, so far (attn_launch_tag)
 
 constexpr int kWorks = 2;  // items handed out ahead
 struct Bars {
@@ -322,6 +323,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 10) {
       // ------------------------------------------------------------------ the pieces
+      AttnPartials ws = p.ws;
+      ws.tag = attn_launch_tag(ws.tag, g_attn_reports);
       const AttnShare share = attn_share(a, g, blockIdx.x, gridDim.x);
       AttnCursor cur;
       bool more = share.u0 < share.u1;
@@ -348,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (found == kNone) break;
         // needed at the piece's end only
         if (found == kPartial)
-          attn_pieces(g, share.line, p.ws, start, keys, (keys + kTile - 1) / kTile, blockIdx.x,
+          attn_pieces(g, share.line, ws, start, keys, (keys + kTile - 1) / kTile, blockIdx.x,
                       toks > g.sub ? 2 : 1, &w->pieces);
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.pieces_full[n % kWorks]);
@@ -824,6 +827,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 }  // namespace
+
+bool count_attn_tc_report() {
+  unsigned v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attn_reports, sizeof(v)) != cudaSuccess) return false;
+  ++v;
+  return cudaMemcpyToSymbol(g_attn_reports, &v, sizeof(v)) == cudaSuccess;
+}
 
 unsigned read_attn_tc_error(bool clear) {
   unsigned v = 0;

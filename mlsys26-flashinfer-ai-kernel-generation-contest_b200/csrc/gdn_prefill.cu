@@ -227,7 +227,9 @@ extern "C" int gdn_device_error(int clear) {
   const unsigned t = gdn::read_selftest_device_error(clear != 0);
   const unsigned x = gdn::read_attn_device_error(clear != 0);
   if (a == ~0u || b == ~0u || d == ~0u || e == ~0u || t == ~0u || x == ~0u) return -1;
-  return (int)(a | b | d | e | t | x);
+  const unsigned bits = a | b | d | e | t | x;
+  if (clear && bits != 0 && !gdn::count_attn_report()) return -1;
+  return (int)bits;
 }
 
 extern "C" int gdn_prefill_launch_strided(

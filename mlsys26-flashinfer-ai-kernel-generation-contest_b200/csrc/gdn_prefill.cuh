@@ -114,7 +114,8 @@ unsigned read_decode_device_error(bool clear);
 unsigned read_segment_device_error(bool clear);
 // Same for the bounded-wait self-test kernel (gdn_selftest_bounded_wait).
 unsigned read_selftest_device_error(bool clear);
-// Same for the attention kernels.
+// Same for the attention kernels, and to be called after a failure was read and cleared.
 unsigned read_attn_device_error(bool clear);
+bool count_attn_report();
 
 }  // namespace gdn

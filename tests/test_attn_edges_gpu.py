@@ -1,8 +1,10 @@
 """GPU: calls of the softmax-attention operators at the edges of what they allow."""
+import ctypes
+
 import pytest
 import torch
 
-from attn_util import check, on, prefill_inputs
+from attn_util import D, check, on, paged_inputs, prefill_inputs
 from conftest import load_pkg
 from oracle import attn_oracle as A
 
@@ -26,3 +28,87 @@ def test_rows_whose_scores_are_all_minus_infinity(cuda, lens):
     assert (out[rows, 1] == 0).all()
     ref[rows, 1], size[rows, 1] = 0, 0
     check(out, ref, size)
+
+
+class _NodeParams(ctypes.Structure):  # CUDA_KERNEL_NODE_PARAMS
+    _fields_ = [("func", ctypes.c_void_p), ("dims", ctypes.c_uint * 7),
+                ("params", ctypes.POINTER(ctypes.c_void_p)), ("extra", ctypes.c_void_p),
+                ("kern", ctypes.c_void_p), ("ctx", ctypes.c_void_p)]
+
+
+def _tag_in(graph, workspace):
+    """The 48-bit number that a captured attention launch marks its words of `workspace` with: it
+    stands behind the addresses of the words and of the partial results."""
+    cu = ctypes.CDLL("libcuda.so.1")
+    n = ctypes.c_size_t()
+    h = ctypes.c_void_p(graph.raw_cuda_graph())
+    assert cu.cuGraphGetNodes(h, None, ctypes.byref(n)) == 0 and n.value == 1
+    node, p = ctypes.c_void_p(), _NodeParams()
+    assert cu.cuGraphGetNodes(h, ctypes.byref(node), ctypes.byref(n)) == 0
+    assert cu.cuGraphKernelNodeGetParams_v2(node, ctypes.byref(p)) == 0
+    info = cu.cuFuncGetParamInfo if p.func else cu.cuKernelGetParamInfo
+    off, size = ctypes.c_size_t(), ctypes.c_size_t()
+    for i in range(8):
+        if info(ctypes.c_void_p(p.func or p.kern), ctypes.c_size_t(i), ctypes.byref(off),
+                ctypes.byref(size)) != 0:
+            break
+        words = (ctypes.c_uint64 * (size.value // 8)).from_address(p.params[i])
+        for j in range(len(words) - 2):
+            if words[j] == workspace.data_ptr():
+                return int(words[j + 2])
+    raise AssertionError("no launch that was given the workspace")
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_replay_after_a_failure_was_reported(cuda, q_len):
+    """What a replay that gave up left in its scratch, words that count some arrivals under the
+    graph's own number, is not taken for arrivals of a replay after gdn_device_error told of the
+    failure (which is made here by the wait that nothing ends)."""
+    pkg = load_pkg()
+    hq, hk, page = 8, 1, 64
+    g = on(paged_inputs([q_len], [30011], hq, hk, page, seed=q_len), cuda)
+    want = pkg.attn_paged(g["q"], g["k_cache"], g["v_cache"], g["table"], g["kv_lens"],
+                          cu_seqlens=g["cu"])
+    need = pkg.LIB.gdn_attn_workspace_size(q_len, 1, hq, hk)
+    ws = torch.zeros(need // 8 + 1, dtype=torch.int64, device=cuda)
+    out = torch.zeros_like(want)
+
+    def launch():
+        k = g["k_cache"]
+        assert pkg.LIB.gdn_attn_paged_launch(
+            g["q"].data_ptr(), k.data_ptr(), g["v_cache"].data_ptr(), g["table"].data_ptr(),
+            g["table"].shape[1], g["kv_lens"].data_ptr(), 0, g["cu"].data_ptr(), 0, 0.0,
+            out.data_ptr(), q_len, 1, g["table"].shape[1], k.shape[0], page, k.stride(0),
+            k.stride(0), hq, hk, D, hq * D, hq * D, ws.data_ptr(), need,
+            torch.cuda.current_stream().cuda_stream) == 0
+    launch()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and pkg.device_error() == 0
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        launch()
+    tag = _tag_in(graph, ws)
+    assert 0 < tag < 2 ** 48
+
+    def left(reports):
+        """The arrivals of some replays that gave up, after so many reports: more than a join waits
+        for (16 pieces a level), so that one which counts on from there never completes."""
+        x = (tag + reports) % 2 ** 48 << 16 | 40
+        return x - 2 ** 64 if x >= 2 ** 63 else x
+
+    def replay(first_words):
+        ws.fill_(-1)  # NaN in the partial results
+        ws[:152 * 2 * 2 * 2] = first_words
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        return torch.equal(out, want)
+    assert replay(-1)  # anything may stand there
+    # not those, before the report (this process may have seen some already)
+    words = next(left(r) for r in range(100) if not replay(left(r)))
+    assert pkg.LIB.gdn_selftest_bounded_wait(1 << 12, 0, None, None) == 0
+    assert pkg.device_error() == 16
+    assert replay(words)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and pkg.device_error() == 0
