@@ -7,14 +7,15 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w              (without weights: y = x)
 //   (y_a, y_b) -> (y_a c_i - y_b s_i, y_b c_i + y_a s_i)   for the rd / 2 pairs
 // with pairs (i, i + rd/2) or, interleaved, (2i, 2i + 1); values from rd on pass through.
-// Everything is fp32 and rounded once, to bf16, at the end.  The angles come from a table
+// Everything is fp32 and rounded once, to bf16, at the end; a row whose squares leave fp32's
+// range is taken times a power of two for its norm.  The angles come from a table
 // because a position times a frequency loses the angle in 32 bits at far positions (a
 // 2^-24 relative error of 10^6 radians is 0.06); the caller computes it once in 64 bits.
 //
 // Bound by HBM: 256 bytes in and out per row, one table row per token.  16 lanes own a row
 // (16-byte accesses); the sum of squares is four shuffles, the partner of a value in the
 // half layout one shuffle when rd / 2 is a multiple of 8, else a pass through shared memory.
-#include "gdn_common.cuh"
+#include "gdn_attn_dev.cuh"
 
 namespace gdn {
 namespace {
@@ -48,11 +49,44 @@ __device__ __forceinline__ float sum16(float x) {
   return x;
 }
 
+// 1 / sqrt(mean(x^2) + eps) of a row, of which each of 16 lanes has eight values.
+__device__ __forceinline__ float inverse_rms(const uint4& v, float eps) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 x = bf2x2_to_f2(w[e]);
+    ss = fmaf(x.x, x.x, ss);
+    ss = fmaf(x.y, x.y, ss);
+  }
+  return rsqrtf(sum16(ss) * (1.f / kHeadDim) + eps);
+}
+
+// A row times a power of two, which is exact, and the norm of that: of a finite row times 2^-70
+// the squares sum to less than 2^123; of a small one times 2^100 they are above 2^-66, as its
+// values are multiples of 2^-133, and sum to less than 2^115.  Not inlined: rare.
+struct Scaled {
+  uint4 v;
+  float norm;
+};
+__device__ __forceinline__ bool in_range(float norm) { return norm > 0.f && norm <= 0x1p46f; }
+__device__ __noinline__ Scaled scaled_row(uint4 v, float norm, float eps) {
+  const float f = in_range(norm) ? 1.f : norm > 0x1p46f ? 0x1p100f : 0x1p-70f;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 x = bf2x2_to_f2(w[e]);
+    const __nv_bfloat162 y = __floats2bfloat162_rn(x.x * f, x.y * f);
+    w[e] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+  return {v, inverse_rms(v, eps * f * f)};
+}
+
 enum RopeLayout { kInterleaved = 0, kHalfAligned = 1, kHalfAny = 2 };
 
 // One half-warp per group of heads of one token, HPG at a time: the table row is read once
 // for the group, a batch's loads are in flight together, and with the batch before's work.
-template <int HPG, int LAYOUT>
+template <int HPG, int LAYOUT, bool kNorm>
 __global__ void __launch_bounds__(256, HPG > 1 ? 3 : 1) rope_kernel(const RopeArgs p) {
   __shared__ float stage[LAYOUT == kHalfAny ? 16 : 1][kHeadDim];
   const int lane = threadIdx.x & 15;
@@ -140,6 +174,31 @@ __global__ void __launch_bounds__(256, HPG > 1 ? 3 : 1) rope_kernel(const RopeAr
     for (int i = 0; i < HPG; ++i) now[i] = raw[i];
     const bool last = ++b == p.batches;
     if (!last) load(h0 + HPG);
+    // 1 / the root mean squares, and where the squares leave fp32's range, or fall below it next
+    // to an eps that does not hide them (their mean is below 2^-92 then), of the row times a
+    // power of two.  One vote for a batch: a branch in each head keeps the heads from overlapping
+    // (32768 tokens 74 us, with this 65.9; products in pairs, without which it is 70.7).
+    float norm[HPG];
+    if constexpr (kNorm) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < HPG; ++i) {
+        norm[i] = inverse_rms(now[i], p.eps);
+        odd |= !in_range(norm[i]);
+      }
+      if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+        for (int i = 0; i < HPG; ++i) {
+          const int h = h0 + i;
+          const bool normed = h < p.hq          ? p.q_weight != nullptr
+                              : h < p.hq + p.hkv ? p.k_weight != nullptr
+                                                 : false;
+          const Scaled z = scaled_row(now[i], normed ? norm[i] : 1.f, p.eps);
+          now[i] = z.v;
+          norm[i] = z.norm;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < HPG; ++i) {
       const int h = h0 + i;
@@ -155,17 +214,18 @@ __global__ void __launch_bounds__(256, HPG > 1 ? 3 : 1) rope_kernel(const RopeAr
         }
       }
       const float* weight = h < p.hq ? p.q_weight : p.k_weight;
-      if (p.q_weight != nullptr || p.k_weight != nullptr) {  // (all lanes take the shuffles)
-        float ss = 0.f;
+      if (kNorm && weight != nullptr && !is_v) {
+        const float r = norm[i];
+        const float4 w0 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane);
+        const float4 w1 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane + 1);
+        const uint64_t r2 = pair(r, r);
+        const uint64_t ww[4] = {pair(w0.x, w0.y), pair(w0.z, w0.w), pair(w1.x, w1.y),
+                                pair(w1.z, w1.w)};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-        ss = sum16(ss);
-        if (weight != nullptr && !is_v) {
-          const float r = rsqrtf(ss * (1.f / kHeadDim) + p.eps);
-          const float4 w0 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane);
-          const float4 w1 = __ldg(reinterpret_cast<const float4*>(weight) + 2 * lane + 1);
-          x[0] *= r * w0.x; x[1] *= r * w0.y; x[2] *= r * w0.z; x[3] *= r * w0.w;
-          x[4] *= r * w1.x; x[5] *= r * w1.y; x[6] *= r * w1.z; x[7] *= r * w1.w;
+        for (int e = 0; e < 4; ++e) {
+          const float2 z = unpair(mul2(pair(x[2 * e], x[2 * e + 1]), mul2(r2, ww[e])));
+          x[2 * e] = z.x;
+          x[2 * e + 1] = z.y;
         }
       }
       float y[8];
@@ -218,15 +278,15 @@ __global__ void __launch_bounds__(256, HPG > 1 ? 3 : 1) rope_kernel(const RopeAr
   }
 }
 
-template <int HPG>
+template <int HPG, bool kNorm>
 cudaError_t launch_rope(const RopeArgs& p, int layout, cudaStream_t st) {
   const unsigned grid = (unsigned)((p.groups + 15) / 16);
   if (layout == kInterleaved)
-    rope_kernel<HPG, kInterleaved><<<grid, 256, 0, st>>>(p);
+    rope_kernel<HPG, kInterleaved, kNorm><<<grid, 256, 0, st>>>(p);
   else if (layout == kHalfAligned)
-    rope_kernel<HPG, kHalfAligned><<<grid, 256, 0, st>>>(p);
+    rope_kernel<HPG, kHalfAligned, kNorm><<<grid, 256, 0, st>>>(p);
   else
-    rope_kernel<HPG, kHalfAny><<<grid, 256, 0, st>>>(p);
+    rope_kernel<HPG, kHalfAny, kNorm><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -311,14 +371,19 @@ extern "C" int gdn_attn_qk_norm_rope_launch(
   p.wide = misaligned(rope_table, 16) == 0 &&
            (interleaved ? rotary_dim % 8 == 0 : layout == kHalfAligned && rotary_dim % 16 == 0);
   // A half-warp takes all heads of a token, four at a time, where there are tokens enough to
-  // fill the card (32768 tokens of 20 heads: 69.8 us, four heads a half-warp 88 us), four
-  // heads where not, and one where even that leaves SMs idle (7 tokens: 3.4 us, four 4.0 us).
+  // fill the card (32768 tokens of 20 heads: 66.6 us, four heads a half-warp 101; 4095: 12.5 and
+  // 13.1; 1777: 9.8 and 8.2), four heads where not, and one where even that leaves SMs idle (7
+  // tokens: 2.5 us, four 3.5; 600: 4.9 and 4.3).
   const int hpg = (long long)num_tokens * heads <= 16 * 148 ? 1 : 4;
   p.batches = num_tokens >= 4096 ? (heads + hpg - 1) / hpg : 1;
   p.groups_per_token = (heads + hpg * p.batches - 1) / (hpg * p.batches);
   const long long groups = (long long)num_tokens * p.groups_per_token;
   if (groups > 0x7fffffffLL) return GDN_ERR_INVALID_ARGUMENT;
   p.groups = (unsigned)groups;
-  const cudaError_t err = hpg == 1 ? launch_rope<1>(p, layout, st) : launch_rope<4>(p, layout, st);
+  const bool norm = q_weight != nullptr || k_weight != nullptr;
+  const cudaError_t err = hpg == 1 ? (norm ? launch_rope<1, true>(p, layout, st)
+                                           : launch_rope<1, false>(p, layout, st))
+                                   : (norm ? launch_rope<4, true>(p, layout, st)
+                                           : launch_rope<4, false>(p, layout, st));
   return err == cudaSuccess ? GDN_OK : GDN_ERR_LAUNCH;
 }

@@ -176,28 +176,6 @@ __device__ __forceinline__ float max_of(const float (&s)[2][32]) {  // NaN if an
   return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
 }
 
-// Two fp32 values in one register pair.
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
-
 // 2^x of a finite pair, below 2^9 (from 2^-126 up; less gives 2^-126), on the FMA pipe: the
 // nearest integer n comes out of the sum with 1.5 2^23, and 2^(x - n) on [-1/2, 1/2] is a
 // cubic, fitted by reweighted least squares to a relative error of 7.5e-5 at most, a

@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from attn_util import D, check, on, paged_inputs, prefill_inputs
+from attn_util import D, check, on, paged_inputs, prefill_inputs, randn
 from conftest import load_pkg
 from oracle import attn_oracle as A
 
@@ -112,3 +112,41 @@ def test_replay_after_a_failure_was_reported(cuda, q_len):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and pkg.device_error() == 0
+
+
+@pytest.mark.parametrize("t,rd,inter", [(12, 64, False), (12, 128, True), (12, 6, False),
+                                        (4101, 64, False)])
+@pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-36])
+def test_norm_of_rows_whose_squares_leave_fp32(cuda, t, rd, inter, eps):
+    """Rows of the largest bf16 values and, with an eps that does not hide them, of the smallest
+    (their squares are beyond or below fp32's range), beside ordinary ones in the same warps; an
+    infinite value gives NaN in its own row alone."""
+    pkg = load_pkg()
+    g0 = torch.Generator().manual_seed(t + rd)
+    hq, hk = 5, 1
+    q, k = randn((t, hq, D), g0, 2.0), randn((t, hk, D), g0, 2.0)
+    top = torch.finfo(torch.bfloat16).max
+    q[0, 0], q[1, 1], q[2, 2] = top, -top, q[2, 2] * 2.0 ** 62
+    q[3, 0], k[3], q[4, 1] = q[3, 0] * 2.0 ** 120, k[3] * 2.0 ** 63, q[4, 1] * 2.0 ** -60
+    q[5, 0], q[6, 1], k[7] = q[5, 0] * 2.0 ** -75, 2.0 ** -133, k[7] * 2.0 ** -130
+    q[8, 0] = 0
+    q[8, 0, 3] = top  # one large value among zeros
+    q[t - 1, hq - 1] = top
+    pos = torch.randint(0, 50, (t,), generator=g0)
+    table = pkg.rope_table(50, rd, device="cpu")
+    w = 1 + 0.3 * torch.randn(D, generator=g0)
+    at = torch.tensor([*range(12), *range(12, t, 97), t - 1])
+    want = [A.norm_rope(x[at], w, pos[at], table, eps=eps, interleaved=inter) for x in (q, k)]
+    # a rotated value is off by at most 16 roundings of |y_a| + |y_b|, of the row's largest twice
+    size = [2 * (x[at].double() * w).abs().amax(-1, keepdim=True)
+            / torch.sqrt((x[at].double() ** 2).mean(-1, keepdim=True) + eps) for x in (q, k)]
+    q[9, 3, 70] = float("inf")
+    args = [x.to(cuda) for x in (q, k, pos, table, w, w)]
+    got = pkg.attn_qk_norm_rope(*args, eps=eps, interleaved=inter)
+    for o, ref, z in zip(got, want, size):
+        o = o.cpu()[at].double()
+        if o.shape[1] == hq:
+            assert not torch.isfinite(o[9, 3]).all()
+            o[9, 3], ref[9, 3] = 0, 0
+        off = (o - ref).abs()
+        assert (off <= 2.0 ** -8 * ref.abs() + 2.0 ** -19 * z + 2.0 ** -133).all()
