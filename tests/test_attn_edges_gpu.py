@@ -1,10 +1,11 @@
 """GPU: calls of the softmax-attention operators at the edges of what they allow."""
 import ctypes
+import threading
 
 import pytest
 import torch
 
-from attn_util import D, check, on, paged_inputs, prefill_inputs, randn
+from attn_util import D, check, on, paged_inputs, paged_ref, prefill_inputs, randn
 from conftest import load_pkg
 from oracle import attn_oracle as A
 
@@ -150,3 +151,63 @@ def test_norm_of_rows_whose_squares_leave_fp32(cuda, t, rd, inter, eps):
             o[9, 3], ref[9, 3] = 0, 0
         off = (o - ref).abs()
         assert (off <= 2.0 ** -8 * ref.abs() + 2.0 ** -19 * z + 2.0 ** -133).all()
+
+
+@pytest.mark.parametrize("page", [200, 208, 256, 1024])
+@pytest.mark.parametrize("hq,hk,q_len", [(4, 4, 1), (16, 2, 1), (8, 1, 2), (16, 2, 4)])
+def test_few_rows_over_large_pages(cuda, page, hq, hk, q_len):
+    """Pages of more rows than all warps take at once."""
+    pkg = load_pkg()
+    d = paged_inputs([q_len] * 5, [q_len, page, page + 1, 3 * page - 1, 2500], hq, hk, page,
+                     seed=page + hq, stale=float("nan"))
+    ref, size = paged_ref(d)
+    g = on(d, cuda)
+    out = pkg.attn_paged(g["q"].view(5, q_len, hq, D), g["k_cache"], g["v_cache"], g["table"],
+                         g["kv_lens"])
+    torch.cuda.synchronize()
+    assert pkg.device_error() == 0
+    check(out, ref, size, f"page {page}")
+
+
+def test_two_threads(cuda):
+    """Calls from two host threads, each on a stream of its own, of shapes that are new to both."""
+    pkg = load_pkg()
+    made = []
+    for i in range(2):
+        p = on(prefill_inputs([333 + i, 70, 5], 4, 2, seed=50 + i), cuda)
+        c = on(paged_inputs([1 + 40 * i] * 3, [900, 77 + i, 41], 4, 2, 16, seed=60 + i), cuda)
+        table = pkg.rope_table(500, 64, device=cuda)
+        pos = torch.arange(p["q"].shape[0], device=cuda)
+        made.append((p, c, table, pos))
+
+    def calls(i):
+        p, c, table, pos = made[i]
+        q, k = pkg.attn_qk_norm_rope(p["q"], p["k"], pos, table)
+        return [q, k, pkg.attn_prefill(q, k, p["v"], p["cu"]),
+                pkg.attn_paged(c["q"], c["k_cache"], c["v_cache"], c["table"], c["kv_lens"],
+                               cu_seqlens=c["cu"])]
+    got, wrong = [[], []], []
+    start = threading.Barrier(2)
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            start.wait(60)
+            with torch.cuda.stream(stream):
+                for _ in range(30):
+                    got[i].append(calls(i))
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    torch.cuda.synchronize()
+    assert not wrong and [len(x) for x in got] == [30, 30] and pkg.device_error() == 0
+    for i in range(2):
+        want = calls(i)
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(want, run))
