@@ -64,9 +64,13 @@ def attn_prefill(q, k, v, cu_seqlens, scale=None, output=None):
     q, k, v and ``output`` may be views whose token rows are strided (slices of a fused
     projection); other layouts go through dense temporaries.
 
-    A token's output does not depend on other sequences, nor, for finite values, on later
-    tokens (a later value that is infinite or NaN can reach the earlier rows of its tile, as
-    0 * inf)."""
+    A token's output does not depend on the values of other sequences, nor, for finite values,
+    on those of later tokens (a later value that is infinite or NaN can reach the earlier rows
+    of its tile, as 0 * inf).  The lengths in the batch decide how its sums are grouped, so its
+    last bits can differ from one batch to another; the same call repeats bit for bit.
+
+    Empty sequences are allowed, but many of them beside a long one cost time: the kernel for
+    few rows is chosen by the mean."""
     try:
         out = torch.empty_like(q) if output is None else output
         plan = _prefill_plans.get(_prefill_key(q, k, v, cu_seqlens, out))
@@ -149,7 +153,8 @@ def attn_paged(q, k_cache, v_cache, block_table, kv_lens, scale=None, output=Non
     A page number outside the cache reads as zeros (nothing is read there), a kv_len above
     width * page_size counts as that.  What lies behind kv_len in a page is not used,
     whatever it holds; as in :func:`attn_prefill`, a newer token's infinite or NaN value can
-    reach older rows of its tile."""
+    reach older rows of its tile, the batch's lengths decide how sums are grouped, and a packed
+    batch of mostly empty sequences costs time."""
     try:
         out = torch.empty_like(q) if output is None else output
         plan = _paged_plans.get(_paged_key(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens,

@@ -42,7 +42,11 @@ int parts() {
 // ragged a packed batch is.  One chunk among single tokens would be read by many small items,
 // so past 32 items in the longest sequence that is possible the tensor cores take it (255
 // single tokens and a chunk of 512 over 16384 keys, 8 / 8 heads: 329 us, few rows 604; below,
-// 63 and a chunk of 256 over 8192: few rows 219, the other 295).
+// 63 and a chunk of 256 over 8192: few rows 219, the other 295).  Possible with a token in every
+// sequence: empty ones void that bound (16 / 2 heads: a prompt of 1000 tokens with 999 empty
+// sequences 188 us, alone 31; a chunk of 1000 over 8192 keys 619 and 85).  Without counting on
+// those tokens every packed batch of more than 32 single tokens, 16 / 2 heads, would go to the
+// tensor cores.
 int few_rows(long long total_q, int num_seqs, int hq, int hkv, bool uniform) {
   const int grp = hq / hkv;
   const long long mean = (total_q + num_seqs - 1) / num_seqs * grp;

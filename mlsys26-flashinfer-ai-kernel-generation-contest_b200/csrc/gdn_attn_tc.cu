@@ -18,8 +18,9 @@
 // Bound by the chain of each row tile, scores -> TMEM read -> maximum -> exponentials -> P ->
 // product, of which two are in flight: for 128 keys of both tiles the products take 2048 clocks
 // and the exponentials 2048 (16 a clock; 1536 with a quarter of them on the FMA pipe), and the
-// pipes are 55 % and 45 % busy.  One prompt of 16384 tokens (16 / 2 heads): 0.93 to 0.99 ms by
-// the clock that the power limit leaves, 1.1 to 1.2 PFLOP/s (cuBLAS 1.68).
+// pipes are 55 % and 45 % busy.  One prompt of 16384 tokens (16 / 2 heads): 0.91 to 0.96 ms in
+// bursts, 1.15 to 1.21 PFLOP/s (cuBLAS 1.68), and 1.04 to 1.09 call after call, 1.01 to 1.06
+// (cuBLAS 1.39): the power limit leaves 1650 of 1965 MHz.
 //
 // The maximum that a row's sums are relative to is raised only when the new one exceeds it
 // by 2^8: P then stays below 2^8 and the sums in fp32 lose nothing, and the rescaling of O

@@ -226,7 +226,8 @@ def attn_append(q, k, v, positions, rope_table, slots, k_cache, v_cache, q_weigh
     ``v_cache`` [num_pages, page_size, HK, 128] (bf16, updated in place; pages may be
     strided).  Returns ``q_out`` (may be q).
 
-    Slots must be distinct.  A slot outside the cache writes nothing there; a token whose
+    Any page size is written; :func:`attn_paged` reads pages of a multiple of 8 rows.  Slots must
+    be distinct.  A slot outside the cache writes nothing there; a token whose
     position lies outside the table is padding: zeros in q_out, nothing in the cache."""
     if k_cache is None:
         raise TypeError("k_cache must be a torch.Tensor, got NoneType")
