@@ -480,8 +480,8 @@ int gdn_attn_prefill_launch(const void* q, const void* k, const void* v, const v
  * pages of each sequence in order; kv_lens int32 or int64 [num_seqs]: its tokens, the new
  * ones included (at most table_width * page_size are used).  Token i of q_len sees the
  * first kv_len - q_len + i + 1 tokens; one that sees none, or all of whose scores are -inf
- * (as for whole prompts), gets zeros.  A page number outside [0, num_pages) reads as zeros.  What lies behind kv_len in a page is not used,
- * whatever it holds.
+ * (as for whole prompts), gets zeros.  A page number outside [0, num_pages) reads as zeros.
+ * What lies behind kv_len in a page is not used, whatever it holds.
  */
 int gdn_attn_paged_launch(const void* q, const void* k_cache, const void* v_cache,
                           const int* block_table, long long block_table_stride,
